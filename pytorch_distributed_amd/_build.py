@@ -29,6 +29,9 @@ CSRC = PKG / "csrc"
 LIB = PKG / "lib"
 OBJ = PKG / "build"
 ARCH = "gfx950"
+# No packed fp32 arithmetic (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32): hipcc -O3 forms it from ordinary float code, and some
+# of its forms have given wrong results on MI355X now and then, without an error.
+HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 HIPCC = os.environ.get("PDA_HIPCC") or shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 CXX = os.environ.get("PDA_CXX") or shutil.which("g++") or "g++"
@@ -65,13 +68,14 @@ def _mark(target: Path, stamp: str) -> None:
 def build_kernels(force: bool = False, jobs: int | None = None, verbose: bool = False) -> Path:
     srcs = sorted((CSRC / "kernels").glob("*.hip"))
     hdrs = sorted((CSRC / "kernels").glob("*.h"))
-    stamp = _stamp(srcs + hdrs)
+    flags = hashlib.sha1(" ".join(HIP_FLAGS).encode()).hexdigest()
+    stamp = _stamp(srcs + hdrs) + flags
     if not force and not _needs(KERNEL_LIB, stamp):
         return KERNEL_LIB
     LIB.mkdir(exist_ok=True)
     OBJ.mkdir(exist_ok=True)
     jobs = jobs or min(8, os.cpu_count() or 4, int(os.environ.get("MAX_JOBS", "8")))
-    hstamp = _stamp(hdrs)
+    hstamp = _stamp(hdrs) + flags
 
     def one(src: Path) -> Path:
         obj = OBJ / (src.stem + ".o")
@@ -79,7 +83,7 @@ def build_kernels(force: bool = False, jobs: int | None = None, verbose: bool = 
         if force or _needs(obj, st):
             if verbose:
                 print("[pda build] hipcc", src.name, flush=True)
-            _run([HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+            _run([HIPCC, f"--offload-arch={ARCH}", *HIP_FLAGS,
                   "-I", str(CSRC / "kernels"), "-c", str(src), "-o", str(obj)])
             _mark(obj, st)
         return obj
@@ -105,7 +109,7 @@ def build_variant(name: str, defines, verbose: bool = False) -> Path:
         obj = objdir / (src.stem + ".o")
         if verbose:
             print("[pda build]", name, src.name, flush=True)
-        _run([HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+        _run([HIPCC, f"--offload-arch={ARCH}", *HIP_FLAGS,
               "-I", str(CSRC / "kernels"), *[f"-D{d}" for d in defines], "-c", str(src), "-o", str(obj)])
         return obj
 
