@@ -1,0 +1,468 @@
+// Distillation from a teacher's top logits: the selection of a row's k largest logits (with the log-sum-exp of the others)
+// and the Kullback-Leibler loss of a student against them, forward and backward.
+//
+// Rows have one stride, their elements are adjacent; a row starts anywhere (odd class counts), so the 16-byte accesses
+// are typed as element-aligned.  One block takes one row; sums of a row's terms are fp32 over a few hundred elements a
+// thread, what the loss is made of (k entries and three log-sum-exps a row) is fp64: student and teacher are nearly equal
+// late in training and their logarithms cancel.
+#include "common.h"
+
+#include <float.h>
+
+namespace {
+
+constexpr int MAX_K = 1024;          // entries of a row
+constexpr int MAX_CLASSES = 1 << 20;  // one bit a class in shared memory
+
+template <typename T> struct RowVec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+template <typename T>
+__device__ __forceinline__ RowVec<T> row_ld(const T* p) {
+  RowVec<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void row_st(T* p, const RowVec<T>& r) { __builtin_memcpy(p, &r, 16); }
+
+// Running maximum (raw logit) and sum of exp((z - m)/T).  m starts at the lowest finite number, so that neither a row of
+// infinities nor a difference of two of them makes a NaN that the row has not got.
+struct MaxSum {
+  float m, s;
+};
+// exp((z - m)/T) with c = log2(e)/T; 1 for m itself, an infinite one too
+__device__ __forceinline__ float ms_exp(float z, float m, float c) { return z == m ? 1.f : exp2f((z - m) * c); }
+__device__ __forceinline__ void ms_merge(MaxSum& a, float m2, float s2, float c) {
+  const float m = fmaxf(a.m, m2);
+  a.s = a.s * ms_exp(a.m, m, c) + s2 * ms_exp(m2, m, c);
+  a.m = m;
+}
+__device__ __forceinline__ void ms_add(MaxSum& a, float z, float c) {
+  if (z > a.m) {
+    a.s *= exp2f((a.m - z) * c);
+    a.m = z;
+  }
+  a.s += ms_exp(z, a.m, c);
+}
+template <int NT>
+__device__ __forceinline__ MaxSum ms_block(MaxSum a, float c, float* scratch /* 2*NT/64 */) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) ms_merge(a, __shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), c);
+  const int wid = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    scratch[2 * wid] = a.m;
+    scratch[2 * wid + 1] = a.s;
+  }
+  __syncthreads();
+  MaxSum r{scratch[0], scratch[1]};
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) ms_merge(r, scratch[2 * w], scratch[2 * w + 1], c);
+  return r;
+}
+
+// ------------------------------------------------------------------------------------------------ top logits
+// A value as a whole number of the same order: NaN above everything, -0 equal to +0.  0 is below every value.
+__device__ __forceinline__ unsigned order_key(float v) {
+  const unsigned b = __float_as_uint(v);
+  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  if ((b << 1) == 0u) return 0x80000000u;
+  return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+}
+
+// The digit (0..255) at which a count from the top (or, with ascending, from the bottom) reaches need; need becomes what
+// is still to be taken inside that digit.  hist[256] -> every thread.
+template <int NT>
+__device__ __forceinline__ int radix_digit(unsigned* hist, int& need, bool ascending, int* out /* 2 ints */) {
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int l = threadIdx.x;
+    int h[4], own = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = l * 4 + i;
+      h[i] = (int)hist[ascending ? d : 255 - d];
+      own += h[i];
+    }
+    int before = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(before, o, 64);
+      if (l >= o) before += t;
+    }
+    before -= own;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (before < need && need <= before + h[i]) {
+        out[0] = ascending ? l * 4 + i : 255 - (l * 4 + i);
+        out[1] = need - before;
+      }
+      before += h[i];
+    }
+  }
+  __syncthreads();
+  need = out[1];
+  return out[0];
+}
+
+// One block a row.  The k-th largest key is found digit by digit (a histogram of 256 counts a pass over the row), then,
+// where more values equal it than are wanted, the highest class that still belongs, digit by digit of the class; the k
+// elements are gathered and ranked by counting.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT)
+top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, double temperature, T* __restrict__ values,
+                  long long* __restrict__ indices, float* __restrict__ rest) {
+  __shared__ unsigned hist[256];
+  __shared__ int pick[2];
+  __shared__ int count;
+  __shared__ float scratch[2 * NT / 64];
+  __shared__ unsigned long long cand[MAX_K];
+  const T* row = z + (long long)blockIdx.x * ld;
+  unsigned key = 0;
+  int need = K;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = threadIdx.x; i < 256; i += NT) hist[i] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < V; j += NT) {
+      const unsigned q = order_key(ElemTraits<T>::to_f32(row[j]));
+      if (shift == 24 || (q >> (shift + 8)) == key) atomicAdd(&hist[(q >> shift) & 255], 1u);
+    }
+    key = (key << 8) | (unsigned)radix_digit<NT>(hist, need, false, pick);
+    __syncthreads();
+  }
+  // need of the elements that equal key are wanted, those of the lowest classes
+  unsigned last = 0;
+  int top_shift = 0;
+  while (((V - 1) >> top_shift) > 255) top_shift += 8;
+  for (int shift = top_shift; shift >= 0; shift -= 8) {
+    for (int i = threadIdx.x; i < 256; i += NT) hist[i] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < V; j += NT) {
+      if (order_key(ElemTraits<T>::to_f32(row[j])) != key) continue;
+      if (shift == top_shift || ((unsigned)j >> (shift + 8)) == last) atomicAdd(&hist[((unsigned)j >> shift) & 255], 1u);
+    }
+    last = (last << 8) | (unsigned)radix_digit<NT>(hist, need, true, pick);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  MaxSum ms{-FLT_MAX, 0.f};
+  for (int j = threadIdx.x; j < V; j += NT) {
+    const float v = ElemTraits<T>::to_f32(row[j]);
+    const unsigned q = order_key(v);
+    if (q > key || (q == key && (unsigned)j <= last)) {
+      const int p = atomicAdd(&count, 1);
+      if (p < MAX_K) cand[p] = ((unsigned long long)q << 32) | (0xffffffffu - (unsigned)j);
+    } else {
+      ms_add(ms, v, c);
+    }
+  }
+  ms = ms_block<NT>(ms, c, scratch);  // its barriers also close the list of candidates
+  for (int i = threadIdx.x; i < K; i += NT) {
+    const unsigned long long me = cand[i];
+    int r = 0;
+    for (int o = 0; o < K; ++o) r += cand[o] > me ? 1 : 0;
+    const unsigned j = 0xffffffffu - (unsigned)me;
+    values[(long long)blockIdx.x * K + r] = row[j];
+    indices[(long long)blockIdx.x * K + r] = (long long)j;
+  }
+  if (threadIdx.x == 0)
+    rest[blockIdx.x] = ms.s == 0.f ? -INFINITY : (float)((double)ms.m / temperature + log((double)ms.s));
+}
+
+// ------------------------------------------------------------------------------------------------ distillation loss
+__device__ __forceinline__ float rd_value(const void* p, int dtype, long long i) {
+  if (dtype == PDA_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == PDA_F16) return (float)reinterpret_cast<const f16*>(p)[i];
+  return (float)reinterpret_cast<const bf16*>(p)[i];
+}
+__device__ __forceinline__ long long rd_index(const void* p, int is64, long long i) {
+  return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
+}
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// maximum that keeps a NaN
+__device__ __forceinline__ double max_nan(double a, double b) { return (b > a || b != b) ? b : a; }
+__device__ __forceinline__ double wave_max_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max_nan(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// What a row leaves for its backward pass: dz_j = T (exp((z_j - shift)/T) * factor) g outside the entries, T dtop_k g at
+// entry k (dtop = q - p).  A factor of 0 is a row whose gradient is zero everywhere outside the entries.
+struct RowStat { float shift, factor; };
+
+// Shared memory of a row: the entries, then one bit a class.
+struct RowEntries {
+  double* p;        // [K] teacher probabilities
+  int* idx;         // [K] class, -1 for an empty entry
+  int* first;       // [K] the first entry of the same class
+  float* z;         // [K] the student's logit there
+  unsigned* bits;   // [(V + 31)/32]
+  __device__ RowEntries(char* mem, int K) {
+    p = reinterpret_cast<double*>(mem);
+    idx = reinterpret_cast<int*>(mem + 8ll * K);
+    first = idx + K;
+    z = reinterpret_cast<float*>(first + K);
+    bits = reinterpret_cast<unsigned*>(z + K);
+  }
+};
+inline size_t row_entries_bytes(int K, int V) { return 20ull * K + 4ull * ((V + 31) / 32) + 16; }
+
+// With rest, classes that are entries stay out of (m, s): the student's remainder is summed by itself, since one minus
+// the entries' sum would keep no digits where the entries hold nearly everything.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT)
+distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __restrict__ values, int vdtype, long long vld,
+                   const void* __restrict__ indices, int idx64, long long ild, const float* __restrict__ rest, int K,
+                   double temperature, float c, float* __restrict__ row_loss, RowStat* __restrict__ stat,
+                   float* __restrict__ dtop) {
+  extern __shared__ __align__(16) char mem[];
+  __shared__ float scratch[2 * NT / 64];
+  __shared__ int twice;
+  const RowEntries en(mem, K);
+  const long long rowi = blockIdx.x;
+  const T* row = z + rowi * ld;
+  constexpr int VN = RowVec<T>::N;
+  for (int i = threadIdx.x; i < (V + 31) / 32; i += NT) en.bits[i] = 0u;
+  if (threadIdx.x == 0) twice = 0;
+  __syncthreads();
+  for (int k = threadIdx.x; k < K; k += NT) {
+    const long long i = rd_index(indices, idx64, rowi * ild + k);
+    const int j = (i >= 0 && i < V) ? (int)i : -1;
+    en.idx[k] = j;
+    en.first[k] = k;
+    if (j >= 0) {
+      en.z[k] = ElemTraits<T>::to_f32(row[j]);
+      if (atomicOr(&en.bits[j >> 5], 1u << (j & 31)) & (1u << (j & 31))) twice = 1;
+    }
+  }
+  __syncthreads();
+  MaxSum ms{-FLT_MAX, 0.f};
+  const int nv = V / VN;
+  const unsigned char* bytes = reinterpret_cast<const unsigned char*>(en.bits);
+  for (int i = threadIdx.x; i < nv; i += NT) {
+    const RowVec<T> v = row_ld(row + (long long)i * VN);
+    unsigned skip = 0;
+    if (rest) skip = VN == 8 ? bytes[i] : (bytes[i >> 1] >> ((i & 1) * 4)) & 15u;
+#pragma unroll
+    for (int e = 0; e < VN; ++e)
+      if (!((skip >> e) & 1u)) ms_add(ms, ElemTraits<T>::to_f32(v.v[e]), c);
+  }
+  for (int j = nv * VN + threadIdx.x; j < V; j += NT)
+    if (!rest || !((en.bits[j >> 5] >> (j & 31)) & 1u)) ms_add(ms, ElemTraits<T>::to_f32(row[j]), c);
+  ms = ms_block<NT>(ms, c, scratch);
+  if (twice)  // rare: entries of one class are one class of the distribution
+    for (int k = threadIdx.x; k < K; k += NT)
+      if (en.idx[k] >= 0)
+        for (int o = 0; o < k; ++o)
+          if (en.idx[o] == en.idx[k]) { en.first[k] = o; break; }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const int lane = threadIdx.x;
+  const double it = 1.0 / temperature;
+  // student: L = log sum exp(z/T) over everything, lt over the remainder (with rest)
+  // (a softmax that holds +inf is NaN, as everywhere else)
+  const double lt = ms.m == INFINITY ? (double)NAN : (double)ms.m * it + log((double)ms.s);
+  double L = lt;
+  if (rest) {
+    double m = -DBL_MAX;
+    for (int k = lane; k < K; k += 64)
+      if (en.idx[k] >= 0) m = max_nan(m, (double)en.z[k] * it);
+    m = wave_max_d(m);
+    double s = 0.0;
+    for (int k = lane; k < K; k += 64)
+      if (en.idx[k] >= 0 && en.first[k] == k) s += exp((double)en.z[k] * it - m);
+    s = wave_sum_d(s);
+    const double le = m + log(s), hi = max_nan(le, lt);
+    L = hi + log(exp(le - hi) + exp(lt - hi));
+  }
+  // teacher
+  const double R = rest ? (double)rest[rowi] : -INFINITY;
+  double tm = -INFINITY;
+  int any = 0;
+  for (int k = lane; k < K; k += 64)
+    if (en.idx[k] >= 0) {
+      any = 1;
+      tm = max_nan(tm, (double)rd_value(values, vdtype, rowi * vld + k) * it);
+    }
+  any = __any(any);
+  tm = max_nan(wave_max_d(tm), R);
+  if (!any || tm == -INFINITY) {  // nothing to learn from
+    for (int k = lane; k < K; k += 64) dtop[rowi * K + k] = 0.f;
+    if (lane == 0) {
+      row_loss[rowi] = 0.f;
+      stat[rowi] = RowStat{0.f, 0.f};
+    }
+    return;
+  }
+  double ts = 0.0;
+  for (int k = lane; k < K; k += 64)
+    if (en.idx[k] >= 0) ts += exp((double)rd_value(values, vdtype, rowi * vld + k) * it - tm);
+  ts = wave_sum_d(ts);
+  if (rest) ts += exp(R - tm);
+  const double lz = tm + log(ts);
+  for (int k = lane; k < K; k += 64)
+    en.p[k] = en.idx[k] >= 0 ? exp((double)rd_value(values, vdtype, rowi * vld + k) * it - lz) : 0.0;
+  __threadfence_block();  // read across the wave's lanes below
+  __builtin_amdgcn_wave_barrier();
+  double loss = 0.0;
+  for (int k = lane; k < K; k += 64) {
+    const int j = en.idx[k];
+    double d = 0.0;
+    if (j >= 0) {
+      double p = en.p[k], lp = (double)rd_value(values, vdtype, rowi * vld + k) * it - lz;
+      if (twice) {
+        p = 0.0;
+        for (int o = 0; o < K; ++o)
+          if (en.idx[o] == j) p += en.p[o];
+        lp = log(p);
+      }
+      const double lq = (double)en.z[k] * it - L;
+      if (en.first[k] == k && p != 0.0) loss += p * (lp - lq);
+      d = exp(lq) - p;
+    }
+    dtop[rowi * K + k] = (float)d;
+  }
+  loss = wave_sum_d(loss);
+  // q of the remainder against its own maximum: q_j = exp((z_j - m)/T) * alpha
+  double factor = exp((double)ms.m * it - L);
+  if (rest) {
+    const double pr = exp(R - lz);
+    if (pr != 0.0) {
+      loss += pr * ((R - lz) - (lt - L));
+      factor -= pr / (double)ms.s;
+    }
+    if (ms.s == 0.f) factor = 0.0;
+  }
+  if (lane == 0) {
+    row_loss[rowi] = (float)(loss * temperature * temperature);
+    stat[rowi] = RowStat{ms.m, (float)factor};
+  }
+}
+
+// dz of a row: one value for every class, then the entries' own over it (the barrier orders the two writes).
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT)
+distill_bwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __restrict__ indices, int idx64, long long ild,
+                   int K, float c, const RowStat* __restrict__ stat, const float* __restrict__ dtop,
+                   const float* __restrict__ g, int gstride, float gscale, T* __restrict__ dz) {
+  const long long rowi = blockIdx.x;
+  const T* row = z + rowi * ld;
+  T* out = dz + rowi * V;
+  constexpr int VN = RowVec<T>::N;
+  const float gr = g[rowi * gstride] * gscale;
+  const RowStat st = stat[rowi];
+  const float f = st.factor * gr;
+  const int nv = V / VN;
+  if (st.factor == 0.f) {  // not read: what stands in a row without entries may be anything
+    RowVec<T> v;
+#pragma unroll
+    for (int e = 0; e < VN; ++e) v.v[e] = ElemTraits<T>::from_f32(0.f);
+    for (int i = threadIdx.x; i < nv; i += NT) row_st(out + (long long)i * VN, v);
+    for (int j = nv * VN + threadIdx.x; j < V; j += NT) out[j] = ElemTraits<T>::from_f32(0.f);
+  } else {
+    for (int i = threadIdx.x; i < nv; i += NT) {
+      RowVec<T> v = row_ld(row + (long long)i * VN);
+#pragma unroll
+      for (int e = 0; e < VN; ++e)
+        v.v[e] = ElemTraits<T>::from_f32(exp2f((ElemTraits<T>::to_f32(v.v[e]) - st.shift) * c) * f);
+      row_st(out + (long long)i * VN, v);
+    }
+    for (int j = nv * VN + threadIdx.x; j < V; j += NT)
+      out[j] = ElemTraits<T>::from_f32(exp2f((ElemTraits<T>::to_f32(row[j]) - st.shift) * c) * f);
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < K; k += NT) {
+    const long long j = rd_index(indices, idx64, rowi * ild + k);
+    if (j >= 0 && j < V) out[j] = ElemTraits<T>::from_f32(dtop[rowi * K + k] * gr);
+  }
+}
+
+// out = scale * sum of x: one block, fp64.
+__global__ void __launch_bounds__(1024)
+row_total_kernel(const float* __restrict__ x, long long n, double scale, float* __restrict__ out) {
+  __shared__ double red[16];
+  double a = 0.0;
+  for (long long i = threadIdx.x; i < n; i += 1024) a += (double)x[i];
+  a = wave_sum_d(a);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) a += red[w];
+    *out = (float)(a * scale);
+  }
+}
+
+}  // namespace
+
+#define DISTILL_DISPATCH(dtype, ...)                        \
+  switch (dtype) {                                          \
+    case PDA_F32: { typedef float T; __VA_ARGS__; } break;  \
+    case PDA_F16: { typedef f16 T; __VA_ARGS__; } break;    \
+    case PDA_BF16: { typedef bf16 T; __VA_ARGS__; } break;  \
+    default: return -6;                                     \
+  }
+
+static const double LOG2E = 1.4426950408889634;
+
+PDA_EXPORT int pda_top_logits(int dtype, const void* z, long long ld, long long rows, int V, int K, double temperature,
+                              void* values, long long* indices, float* rest, hipStream_t st) {
+  if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || K <= 0 || K > V || K > MAX_K || !(temperature > 0.0)) return -1;
+  const float c = (float)(LOG2E / temperature);
+  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, (const T*)z,
+                                             ld, V, K, c, temperature, (T*)values, indices, rest));
+  return pda_check_launch();
+}
+
+template <typename T, int NT>
+static int launch_distill_fwd(const void* z, long long ld, long long rows, int V, const void* values, int vdtype,
+                              long long vld, const void* indices, int idx64, long long ild, const float* rest, int K,
+                              double temperature, float* row_loss, void* stat, float* dtop, hipStream_t st) {
+  const size_t lds = row_entries_bytes(K, V);
+  if (lds > 64 * 1024) {
+    hipError_t r = hipFuncSetAttribute(reinterpret_cast<const void*>(distill_fwd_kernel<T, NT>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (r != hipSuccess) return (int)r;
+  }
+  hipLaunchKernelGGL((distill_fwd_kernel<T, NT>), dim3((unsigned)rows), dim3(NT), lds, st, (const T*)z, ld, V, values, vdtype,
+                     vld, indices, idx64, ild, rest, K, temperature, (float)(LOG2E / temperature), row_loss, (RowStat*)stat,
+                     dtop);
+  return pda_check_launch();
+}
+
+// stat: {fp32 shift, fp32 factor} [rows]; dtop: fp32 [rows][K].  loss (may be null): scale * sum of row_loss.
+PDA_EXPORT int pda_distill_fwd(int dtype, const void* z, long long ld, long long rows, int V, const void* values, int vdtype,
+                               long long vld, const void* indices, int idx64, long long ild, const float* rest, int K,
+                               double temperature, float* row_loss, void* stat, float* dtop, float* loss, double scale,
+                               hipStream_t st) {
+  if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || V > MAX_CLASSES || K <= 0 || K > MAX_K || !(temperature > 0.0)) return -1;
+  if (vdtype != PDA_F32 && vdtype != PDA_F16 && vdtype != PDA_BF16) return -6;
+  int rc = 0;
+  DISTILL_DISPATCH(dtype, rc = launch_distill_fwd<T, 256>(z, ld, rows, V, values, vdtype, vld, indices, idx64, ild, rest, K,
+                                                          temperature, row_loss, stat, dtop, st));
+  if (rc == 0 && loss) {
+    hipLaunchKernelGGL(row_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, rows, scale, loss);
+    rc = pda_check_launch();
+  }
+  return rc;
+}
+
+// g: fp32, one for all rows (gstride 0) or one a row (gstride 1); gscale: what it is multiplied with.
+PDA_EXPORT int pda_distill_bwd(int dtype, const void* z, long long ld, long long rows, int V, const void* indices, int idx64,
+                               long long ild, int K, double temperature, const void* stat, const float* dtop, const float* g,
+                               int gstride, float gscale, void* dz, hipStream_t st) {
+  if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || V > MAX_CLASSES || K <= 0 || K > MAX_K || !(temperature > 0.0)) return -1;
+  const float c = (float)(LOG2E / temperature);
+  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st,
+                                             (const T*)z, ld, V, indices, idx64, ild, K, c, (const RowStat*)stat, dtop, g,
+                                             gstride, gscale, (T*)dz));
+  return pda_check_launch();
+}

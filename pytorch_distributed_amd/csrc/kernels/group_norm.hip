@@ -1,0 +1,494 @@
+// Group norm with an optional residual and activation, channels last: x [N][S][C], C = G groups of D channels, m = S*D.
+//   mu, var over the m elements of a (sample, group); r = 1/sqrt(var + eps); xh = (x - mu) r
+//   z = xh*gamma_c + beta_c + res;  out = act(z), act = identity | max(z, 0) | min(max(z, 0), cap) | z*sigmoid(z)
+// Backward with g = dout*act'(z) (z is computed again from x and res, nothing of it is kept):
+//   dres = g,  dbeta_c = sum_{n,s} g,  dgamma_c = sum_{n,s} g xh
+//   A = sum_{group} gamma g, B = sum_{group} gamma g xh;  dx = r (gamma g - (A + xh B)/m)
+//
+// Statistics: a thread takes its rows in batches of four, relative to the first row of its chunk (a mean far from zero
+// costs no digits), forms each batch's mean and centred squares in fp32 and adds batches up in fp64; (sample, group)
+// totals are fp64 and kept as pairs {mu, r}.  16-bit inputs lose nothing in a batch, so their statistics are good to far
+// below fp32: the side of an activation's border on which a value lies can be decided from them (gn_grad).  The element
+// passes take mu as an fp32 pair (hi subtracted from x, lo folded into the shift).
+//
+// Memory-bound throughout: the work is split over (sample, row chunk), a thread owns one vector of channels and walks
+// rows, so the per-channel coefficients stay in registers.  No atomics: results repeat bit for bit.
+#include "common.h"
+
+#include <initializer_list>
+
+namespace {
+
+enum GnAct : int { GN_NONE = 0, GN_RELU = 1, GN_CAP = 2, GN_SILU = 3 };
+
+struct GnStat { double mean, rstd; };
+
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) GnVec { T v[VEC]; };
+
+template <typename T, int VEC>
+__device__ __forceinline__ GnVec<T, VEC> gn_ld(const T* p) { return *reinterpret_cast<const GnVec<T, VEC>*>(p); }
+template <typename T, int VEC>
+__device__ __forceinline__ void gn_st(T* p, const GnVec<T, VEC>& v) { *reinterpret_cast<GnVec<T, VEC>*>(p) = v; }
+
+// Where a block's threads stand: VT vectors of channels side by side, RS rows at a time (threads beyond VT*RS idle).
+struct GnGeom {
+  int VT, RS, col, rl;
+  __device__ explicit GnGeom(int vpr) {
+    VT = vpr < 256 ? vpr : 256;
+    RS = 256 / VT;
+    col = threadIdx.x % VT;
+    rl = threadIdx.x / VT;
+  }
+};
+
+// Sums of one channel over some rows, relative to a pivot: a = sum (x - pivot), b = sum (x - pivot)^2.
+struct GnSums { double a, b; };
+
+// Four values of a channel (or one) added to its sums.  b takes the squares around the batch's own mean and that mean's
+// square in fp64, so a pivot far out (an outlier in the first row) costs no digits of the spread.
+__device__ __forceinline__ void gn_add4(GnSums& s, const float (&f)[4]) {
+  const float mb = ((f[0] + f[1]) + (f[2] + f[3])) * 0.25f;
+  float q = 0.f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) { const float d = f[u] - mb; q += d * d; }
+  const double m4 = (double)mb * 4.0;
+  s.a += m4;
+  s.b += (double)q + m4 * (double)mb;
+}
+__device__ __forceinline__ void gn_add1(GnSums& s, float f) {
+  s.a += (double)f;
+  s.b += (double)f * (double)f;
+}
+
+// Per-channel sums of one row chunk (pivot: its first row) -> part[n][chunk][c].
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+gn_partial_kernel(const T* __restrict__ x, long long S, int C, int chunks, GnSums* __restrict__ part) {
+  __shared__ GnSums sm[256 * VEC];
+  const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
+  const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
+  const int vpr = C / VEC;
+  const GnGeom g(vpr);
+  const T* xn = x + (long long)n * S * C;
+  for (int c0 = 0; c0 < vpr; c0 += g.VT) {
+    const int vec = c0 + g.col;
+    const bool active = g.rl < g.RS && vec < vpr;
+    GnSums s[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s[e] = GnSums{0.0, 0.0};
+    if (active) {
+      const T* p = xn + (long long)vec * VEC;
+      const GnVec<T, VEC> pivot = gn_ld<T, VEC>(p + r0 * C);
+      long long r = r0 + g.rl;
+      for (; r + 3 * g.RS < r1; r += 4 * g.RS) {
+        GnVec<T, VEC> v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = gn_ld<T, VEC>(p + (r + u * g.RS) * C);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float p0 = ElemTraits<T>::to_f32(pivot.v[e]);
+          const float f[4] = {ElemTraits<T>::to_f32(v[0].v[e]) - p0, ElemTraits<T>::to_f32(v[1].v[e]) - p0,
+                              ElemTraits<T>::to_f32(v[2].v[e]) - p0, ElemTraits<T>::to_f32(v[3].v[e]) - p0};
+          gn_add4(s[e], f);
+        }
+      }
+      for (; r < r1; r += g.RS) {
+        const GnVec<T, VEC> v = gn_ld<T, VEC>(p + r * C);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) gn_add1(s[e], ElemTraits<T>::to_f32(v.v[e]) - ElemTraits<T>::to_f32(pivot.v[e]));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sm[e * 256 + threadIdx.x] = s[e];
+    __syncthreads();
+    int h = 1;
+    while (h < g.RS) h <<= 1;
+    for (h >>= 1; h > 0; h >>= 1) {
+      if (g.rl < h && g.rl + h < g.RS) {
+        const int o = threadIdx.x + h * g.VT;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          s[e].a += sm[e * 256 + o].a;
+          s[e].b += sm[e * 256 + o].b;
+          sm[e * 256 + threadIdx.x] = s[e];
+        }
+      }
+      __syncthreads();
+    }
+    if (active && g.rl == 0) {
+      GnSums* o = part + (long long)blockIdx.x * C + (long long)vec * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = s[e];
+    }
+  }
+}
+
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// One wave per (sample, group): chunks x D sums -> {mu, r} in fp64.
+template <typename T>
+__global__ void __launch_bounds__(64)
+gn_finalize_kernel(const T* __restrict__ x, const GnSums* __restrict__ part, long long S, int C, int G, int chunks, double eps,
+                   GnStat* __restrict__ stats) {
+  const int D = C / G;
+  const int n = blockIdx.x / G, g = blockIdx.x % G;
+  const GnSums* p = part + (long long)n * chunks * C + (long long)g * D;
+  const T* xg = x + (long long)n * S * C + (long long)g * D;
+  const long long pairs = (long long)chunks * D;
+  double a = 0.0;
+  for (long long j = threadIdx.x; j < pairs; j += 64) {
+    const int ch = (int)(j / D), d = (int)(j % D);
+    const long long r0 = S * ch / chunks;
+    const double k = (double)(S * (ch + 1) / chunks - r0);
+    a += k * (double)ElemTraits<T>::to_f32(xg[r0 * C + d]) + p[(long long)ch * C + d].a;
+  }
+  const double m = (double)S * D;
+  const double mean = wave_sum_f64(a) / m;
+  double q = 0.0;
+  for (long long j = threadIdx.x; j < pairs; j += 64) {
+    const int ch = (int)(j / D), d = (int)(j % D);
+    const long long r0 = S * ch / chunks;
+    const double k = (double)(S * (ch + 1) / chunks - r0);
+    const GnSums v = p[(long long)ch * C + d];
+    const double own = v.a / k;                       // this channel's mean over the chunk, from the pivot
+    const double e = (double)ElemTraits<T>::to_f32(xg[r0 * C + d]) + own - mean;
+    const double c = v.b - v.a * own;                 // squares around it
+    q += (c > 0.0 ? c : c != c ? c : 0.0) + k * e * e;
+  }
+  q = wave_sum_f64(q);
+  if (threadIdx.x == 0) stats[blockIdx.x] = GnStat{mean, 1.0 / sqrt(q / m + eps)};
+}
+
+// Coefficients of one channel: z = (x - mh)*sc + sh (+ res), xh = (x - mh - ml)*r
+struct GnCoef { float mh, ml, r, sc, sh; };
+__device__ __forceinline__ GnCoef gn_coef(const GnStat& st, float gamma, float beta) {
+  GnCoef k;
+  k.mh = (float)st.mean;
+  k.ml = (float)(st.mean - (double)k.mh);
+  k.r = (float)st.rstd;
+  k.sc = (float)(st.rstd * (double)gamma);
+  k.sh = beta - k.ml * k.sc;
+  return k;
+}
+
+__device__ __forceinline__ float gn_act(float z, int act, float cap) {
+  if (act == GN_SILU) return z / (1.f + __expf(-z));
+  if (act != GN_NONE) z = z < 0.f ? 0.f : z;      // a NaN stays one
+  if (act == GN_CAP) z = z > cap ? cap : z;
+  return z;
+}
+
+// g = dy * act'(z).  A z within rounding of a border of the activation is computed again in fp64 from the fp64
+// statistics: on which side it lies decides over the whole gradient of the element.
+__device__ __forceinline__ float gn_grad(float dy, float x, float res, const GnCoef& k, int act, float cap,
+                                         const GnStat* st, const float* gamma, const float* beta, int c) {
+  if (act == GN_NONE) return dy;
+  const float t = (x - k.mh) * k.sc;
+  const float z = t + k.sh + res;
+  if (act == GN_SILU) {
+    const float s = 1.f / (1.f + __expf(-z));
+    return dy * (s * (1.f + z * (1.f - s)));
+  }
+  const float tol = 1e-6f * (fabsf(t) + fabsf(k.sh) + fabsf(res));
+  bool on = z > 0.f && (act != GN_CAP || z < cap);
+  if (fabsf(z) < tol || (act == GN_CAP && fabsf(z - cap) < tol)) {
+    const double zd = ((double)x - st->mean) * st->rstd * (gamma ? (double)gamma[c] : 1.0) +
+                      (beta ? (double)beta[c] : 0.0) + (double)res;
+    on = zd > 0.0 && (act != GN_CAP || zd < (double)cap);
+  }
+  return on ? dy : 0.f;
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+gn_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ out, const float* __restrict__ gamma,
+                const float* __restrict__ beta, const GnStat* __restrict__ stats, long long S, int C, int G, int chunks,
+                int act, float cap) {
+  const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
+  const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
+  const int vpr = C / VEC, D = C / G;
+  const GnGeom g(vpr);
+  if (g.rl >= g.RS) return;
+  for (int vec = g.col; vec < vpr; vec += g.VT) {
+    GnCoef k[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int c = vec * VEC + e;
+      k[e] = gn_coef(stats[(long long)n * G + c / D], gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
+    }
+    const long long base = (long long)n * S * C + (long long)vec * VEC;
+#pragma unroll 2
+    for (long long r = r0 + g.rl; r < r1; r += g.RS) {
+      const long long o = base + r * C;
+      GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), w;
+      if (res) w = gn_ld<T, VEC>(res + o);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float z = (ElemTraits<T>::to_f32(v.v[e]) - k[e].mh) * k[e].sc + k[e].sh;
+        if (res) z += ElemTraits<T>::to_f32(w.v[e]);
+        v.v[e] = ElemTraits<T>::from_f32(gn_act(z, act, cap));
+      }
+      gn_st<T, VEC>(out + o, v);
+    }
+  }
+}
+
+// Per-channel {sum g, sum g xh} of one row chunk of one sample -> part[n][chunk][c].
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+gn_bwd_partial_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout,
+                      const float* __restrict__ gamma, const float* __restrict__ beta, const GnStat* __restrict__ stats,
+                      long long S, int C, int G, int chunks, int act, float cap, float2* __restrict__ part) {
+  __shared__ float sa[256 * VEC], sb[256 * VEC];
+  const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
+  const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
+  const int vpr = C / VEC, D = C / G;
+  const GnGeom g(vpr);
+  for (int c0 = 0; c0 < vpr; c0 += g.VT) {
+    const int vec = c0 + g.col;
+    const bool active = g.rl < g.RS && vec < vpr;
+    float a[VEC], b[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a[e] = b[e] = 0.f;
+    if (active) {
+      GnCoef k[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int c = vec * VEC + e;
+        k[e] = gn_coef(stats[(long long)n * G + c / D], gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
+      }
+      const long long base = (long long)n * S * C + (long long)vec * VEC;
+#pragma unroll 2
+      for (long long r = r0 + g.rl; r < r1; r += g.RS) {
+        const long long o = base + r * C;
+        const GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), d = gn_ld<T, VEC>(dout + o);
+        GnVec<T, VEC> w;
+        if (res) w = gn_ld<T, VEC>(res + o);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int c = vec * VEC + e;
+          const float xf = ElemTraits<T>::to_f32(v.v[e]);
+          const float gr = gn_grad(ElemTraits<T>::to_f32(d.v[e]), xf, res ? ElemTraits<T>::to_f32(w.v[e]) : 0.f, k[e], act,
+                                   cap, stats + (long long)n * G + c / D, gamma, beta, c);
+          a[e] += gr;
+          b[e] += gr * ((xf - k[e].mh - k[e].ml) * k[e].r);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      sa[e * 256 + threadIdx.x] = a[e];
+      sb[e * 256 + threadIdx.x] = b[e];
+    }
+    __syncthreads();
+    int h = 1;
+    while (h < g.RS) h <<= 1;
+    for (h >>= 1; h > 0; h >>= 1) {
+      if (g.rl < h && g.rl + h < g.RS) {
+        const int o = threadIdx.x + h * g.VT;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          sa[e * 256 + threadIdx.x] = a[e] += sa[e * 256 + o];
+          sb[e * 256 + threadIdx.x] = b[e] += sb[e * 256 + o];
+        }
+      }
+      __syncthreads();
+    }
+    if (active && g.rl == 0) {
+      float2* o = part + (long long)blockIdx.x * C + (long long)vec * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = make_float2(a[e], b[e]);
+    }
+  }
+}
+
+// One wave per (sample, group): {A/m, B/m}.
+__global__ void __launch_bounds__(64)
+gn_bwd_finalize_kernel(const float2* __restrict__ part, const float* __restrict__ gamma, long long S, int C, int G,
+                       int chunks, float2* __restrict__ ab) {
+  const int D = C / G;
+  const int n = blockIdx.x / G, g = blockIdx.x % G;
+  const float2* p = part + (long long)n * chunks * C + (long long)g * D;
+  double a = 0.0, b = 0.0;
+  const long long pairs = (long long)chunks * D;
+  for (long long j = threadIdx.x; j < pairs; j += 64) {
+    const int d = (int)(j % D);
+    const float2 v = p[(j / D) * C + d];
+    const double ga = gamma ? (double)gamma[g * D + d] : 1.0;
+    a += ga * (double)v.x;
+    b += ga * (double)v.y;
+  }
+  a = wave_sum_f64(a);
+  b = wave_sum_f64(b);
+  const double m = (double)S * D;
+  if (threadIdx.x == 0) ab[blockIdx.x] = make_float2((float)(a / m), (float)(b / m));
+}
+
+// dgamma_c, dbeta_c: the column sums of part [rows][C].  A block takes 4 channels with 256 lanes of rows each: with one
+// block a channel group the walk over the rows (thousands at large batch) has to be short.
+__global__ void __launch_bounds__(1024)
+gn_params_kernel(const float2* __restrict__ part, long long rows, int C, float* __restrict__ dgamma,
+                 float* __restrict__ dbeta) {
+  __shared__ double ra[16][4], rb[16][4];
+  const int cl = threadIdx.x & 3, lane = threadIdx.x >> 2;
+  const int c = blockIdx.x * 4 + cl;
+  double a = 0.0, b = 0.0;
+  if (c < C) {
+    long long r = lane;
+    for (; r + 768 < rows; r += 1024) {
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = part[(r + u * 256) * C + c];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) { a += (double)v[u].x; b += (double)v[u].y; }
+    }
+    for (; r < rows; r += 256) {
+      const float2 v = part[r * C + c];
+      a += (double)v.x;
+      b += (double)v.y;
+    }
+  }
+#pragma unroll
+  for (int o = 4; o < 64; o <<= 1) {
+    a += __shfl_xor(a, o, 64);
+    b += __shfl_xor(b, o, 64);
+  }
+  const int wv = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) < 4) { ra[wv][cl] = a; rb[wv][cl] = b; }
+  __syncthreads();
+  if (threadIdx.x < 4 && c < C) {
+#pragma unroll
+    for (int w = 1; w < 16; ++w) { a += ra[w][cl]; b += rb[w][cl]; }
+    dbeta[c] = (float)a;
+    dgamma[c] = (float)b;
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout, T* __restrict__ dx,
+                    T* __restrict__ dres, const float* __restrict__ gamma, const float* __restrict__ beta,
+                    const GnStat* __restrict__ stats, const float2* __restrict__ ab, long long S, int C, int G, int chunks,
+                    int act, float cap) {
+  const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
+  const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
+  const int vpr = C / VEC, D = C / G;
+  const GnGeom g(vpr);
+  if (g.rl >= g.RS) return;
+  for (int vec = g.col; vec < vpr; vec += g.VT) {
+    GnCoef k[VEC];
+    float pa[VEC], pb[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int c = vec * VEC + e;
+      const long long i = (long long)n * G + c / D;
+      k[e] = gn_coef(stats[i], gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
+      const float2 v = ab[i];
+      pa[e] = -v.x * k[e].r;
+      pb[e] = -v.y * k[e].r;
+    }
+    const long long base = (long long)n * S * C + (long long)vec * VEC;
+#pragma unroll 2
+    for (long long r = r0 + g.rl; r < r1; r += g.RS) {
+      const long long o = base + r * C;
+      GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), d = gn_ld<T, VEC>(dout + o), w;
+      if (res) w = gn_ld<T, VEC>(res + o);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int c = vec * VEC + e;
+        const float xf = ElemTraits<T>::to_f32(v.v[e]);
+        const float gr = gn_grad(ElemTraits<T>::to_f32(d.v[e]), xf, res ? ElemTraits<T>::to_f32(w.v[e]) : 0.f, k[e], act, cap,
+                                 stats + (long long)n * G + c / D, gamma, beta, c);
+        const float xh = (xf - k[e].mh - k[e].ml) * k[e].r;
+        v.v[e] = ElemTraits<T>::from_f32(gr * k[e].sc + (pa[e] + xh * pb[e]));
+        d.v[e] = ElemTraits<T>::from_f32(gr);
+      }
+      gn_st<T, VEC>(dx + o, v);
+      if (dres) gn_st<T, VEC>(dres + o, d);
+    }
+  }
+}
+
+// Widest vector (elements) that divides the channels and that every address allows.
+int gn_vec(int C, int esize, std::initializer_list<const void*> ptrs) {
+  for (int vec = 16 / esize; vec > 1; vec >>= 1) {
+    if (C % vec) continue;
+    bool ok = true;
+    for (const void* p : ptrs) ok = ok && reinterpret_cast<uintptr_t>(p) % (size_t)(vec * esize) == 0;
+    if (ok) return vec;
+  }
+  return 1;
+}
+
+bool gn_args_ok(long long N, long long S, int C, int G, int chunks, int act) {
+  return N > 0 && S > 0 && C > 0 && G > 0 && C % G == 0 && chunks > 0 && chunks <= S && act >= GN_NONE && act <= GN_SILU &&
+         N * chunks < (1ll << 31) && N * G < (1ll << 31);
+}
+
+}  // namespace
+
+#define GN_VEC_CASE(T, V, ...) case V: { constexpr int VEC = V; typedef T E; __VA_ARGS__; } break;
+#define GN_DISPATCH(dtype, vec, ...)                                                                     \
+  switch (dtype) {                                                                                        \
+    case PDA_F32: switch (vec) { GN_VEC_CASE(float, 4, __VA_ARGS__) GN_VEC_CASE(float, 2, __VA_ARGS__)                  \
+                                 default: { constexpr int VEC = 1; typedef float E; __VA_ARGS__; } } break;      \
+    case PDA_F16: switch (vec) { GN_VEC_CASE(f16, 8, __VA_ARGS__) GN_VEC_CASE(f16, 4, __VA_ARGS__) GN_VEC_CASE(f16, 2, __VA_ARGS__) \
+                                 default: { constexpr int VEC = 1; typedef f16 E; __VA_ARGS__; } } break;        \
+    case PDA_BF16: switch (vec) { GN_VEC_CASE(bf16, 8, __VA_ARGS__) GN_VEC_CASE(bf16, 4, __VA_ARGS__) GN_VEC_CASE(bf16, 2, __VA_ARGS__) \
+                                  default: { constexpr int VEC = 1; typedef bf16 E; __VA_ARGS__; } } break;      \
+    default: return -6;                                                                                   \
+  }
+
+// Row chunks per sample: about 2048 blocks over the chip, at least 8 rows for each thread of a block.
+PDA_EXPORT int pda_group_norm_chunks(int dtype, long long N, long long S, int C) {
+  if (N <= 0 || S <= 0 || C <= 0) return -1;
+  const int vpr = (C * (dtype == PDA_F32 ? 4 : 2) + 15) / 16;
+  const int rs = vpr >= 256 ? 1 : 256 / vpr;
+  long long want = (2048 + N - 1) / N, most = S / (rs * 8ll);
+  if (want > most) want = most;
+  return (int)(want < 1 ? 1 : want > 1024 ? 1024 : want);
+}
+
+// part: two fp64 [N][chunks][C]; stats: {fp64 mean, fp64 1/std} [N][G]
+PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x, const void* res, void* out, const float* gamma,
+                                  const float* beta, long long N, long long S, int C, int G, double eps, int act, float cap,
+                                  int chunks, void* part, void* stats, hipStream_t st) {
+  if (!gn_args_ok(N, S, C, G, chunks, act)) return -1;
+  const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, out});
+  const int blocks = (int)(N * chunks);
+  GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x, S, C,
+                                             chunks, (GnSums*)part));
+  GN_DISPATCH(dtype, 1, hipLaunchKernelGGL((gn_finalize_kernel<E>), dim3((int)(N * G)), dim3(64), 0, st, (const E*)x,
+                                           (const GnSums*)part, S, C, G, chunks, eps, (GnStat*)stats));
+  GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_apply_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x,
+                                             (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, act,
+                                             cap));
+  return pda_check_launch();
+}
+
+// part: float2 [N][chunks][C]; ab: float2 [N][G].  dgamma / dbeta: both or none.
+PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x, const void* res, const void* dout, void* dx, void* dres,
+                                  const float* gamma, const float* beta, const void* stats, long long N, long long S, int C,
+                                  int G, int act, float cap, int chunks, void* part, void* ab, float* dgamma, float* dbeta,
+                                  hipStream_t st) {
+  if (!gn_args_ok(N, S, C, G, chunks, act) || (dres && !dx)) return -1;
+  const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, dout, dx, dres});
+  const int blocks = (int)(N * chunks);
+  GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_bwd_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x,
+                                             (const E*)res, (const E*)dout, gamma, beta, (const GnStat*)stats, S, C, G, chunks,
+                                             act, cap, (float2*)part));
+  hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const float2*)part, gamma, S, C, G, chunks,
+                     (float2*)ab);
+  if (dgamma)
+    hipLaunchKernelGGL(gn_params_kernel, dim3((C + 3) / 4), dim3(1024), 0, st, (const float2*)part, N * chunks, C, dgamma,
+                       dbeta);
+  if (dx)
+    GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_bwd_apply_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x,
+                                               (const E*)res, (const E*)dout, (E*)dx, (E*)dres, gamma, beta,
+                                               (const GnStat*)stats, (const float2*)ab, S, C, G, chunks, act, cap));
+  return pda_check_launch();
+}

@@ -1,0 +1,311 @@
+"""A teacher's top logits and the distillation loss on them: the kernels against the definition in 64 bits.
+
+Bounds count roundings: u = 2^-24 is half a step of fp32, h half a step of the logits' type.  A log-sum-exp adds at most
+V/256 + 16 terms in a row before the tree, each exponential is off by 4 u and by its argument's rounding (u times its size,
+below 100 in the tests)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from pytorch_distributed_amd import ops
+
+DEV = "cuda"
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+TINY = {torch.float32: 1e-40, torch.float16: 2.0 ** -25, torch.bfloat16: 1e-38}
+INF = float("inf")
+
+
+def logits(rows, V, dtype, seed, scale=3.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn((rows, V), device=DEV, generator=g) * scale).to(dtype)
+
+
+def lse_bound(V):
+    return U * (V / 256 + 16 + 4 + 100)
+
+
+# ------------------------------------------------------------------------------------------------ top logits
+def check_top(z, k, t=1.0):
+    v, i, r = ops.top_logits(z, k, t)
+    order = torch.sort(z.double(), dim=-1, descending=True, stable=True).indices
+    assert i.dtype == torch.int64 and torch.equal(i, order[..., :k])
+    got = z.gather(-1, order[..., :k])
+    assert v.dtype == z.dtype and torch.equal(v.isnan(), got.isnan()) and torch.equal(v[~v.isnan()], got[~got.isnan()])
+    V = z.shape[-1]
+    if V == k:
+        assert bool((r == -INF).all())
+        return
+    want = torch.logsumexp(z.double().gather(-1, order[..., k:]) / t, dim=-1)
+    assert torch.equal(r.isnan(), want.isnan())
+    both = ~want.isnan()
+    r, want = r[both].double(), want[both]
+    same = r == want   # infinities
+    assert bool((same | ((r - want).abs() <= lse_bound(V) + U * want.abs())).all()), float((r - want).abs().max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V,k", [(1, 1, 1), (1, 5, 5), (3, 7, 2), (2, 64, 64), (5, 65, 3), (4, 255, 254), (400, 1000, 10),
+                                      (3, 1000, 1000), (7, 1024, 1024), (3, 4099, 100), (2, 50001, 50), (5, 131072, 64),
+                                      (1, 131073, 1024), (2, 300001, 7), (1, 1 << 20, 128)])
+def test_top_logits_sizes(rows, V, k, dtype):
+    check_top(logits(rows, V, dtype, 1), k, 2.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_top_logits_ties_and_specials(dtype):
+    low = torch.finfo(dtype).min
+    V = 3001
+    z = logits(14, V, dtype, 2)
+    z[0] = 1.0                                   # every value the same
+    z[1] = -INF
+    z[2] = low
+    z[3] = torch.arange(V, device=DEV) % 7       # few values
+    z[4] = torch.linspace(-3, 3, V, device=DEV)  # sorted
+    z[5] = torch.linspace(3, -3, V, device=DEV)
+    z[6, ::2] = -INF
+    z[7, 5:] = -INF                              # fewer values than k
+    z[8, 100:2000] = float("nan")
+    z[9, 77], z[9, 78], z[9, 2000] = INF, INF, float("nan")
+    z[10] = 0.0
+    z[10, ::3] = -0.0
+    z[11, :64] = 50.0                            # one thread's share or the first lanes hold them all
+    z[12, ::256] = 50.0
+    z[13] = -z[13].abs()
+    for k in (1, 12, 64, 300, 1024):
+        check_top(z, k)
+
+
+def test_top_logits_strides_and_leading_dimensions():
+    z = logits(12, 777, torch.bfloat16, 3)
+    check_top(z[:, 5:700], 9)
+    check_top(z[::3, 1:], 9)
+    check_top(z.view(3, 4, 777), 9)
+    check_top(z.view(3, 4, 777).transpose(0, 1), 9)
+    check_top(z.t()[:600], 5)
+    check_top(z[:1].expand(5, 777), 9)
+    v, i, r = ops.top_logits(z[0], 4)
+    assert v.shape == (4,) and r.shape == ()
+    v, i, r = ops.top_logits(z[:0], 4)
+    assert v.shape == (0, 4) and r.shape == (0,)
+
+
+def test_top_logits_repeats_on_other_streams():
+    z = logits(64, 20011, torch.bfloat16, 4)
+    ref = ops.top_logits(z, 33, 2.0)
+    outs = []
+    for s in [torch.cuda.Stream() for _ in range(2)]:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(ops.top_logits(z, 33, 2.0))
+        torch.cuda.current_stream().wait_stream(s)
+    for o in outs:
+        assert torch.equal(o[0], ref[0]) and torch.equal(o[1], ref[1]) and torch.equal(o[2], ref[2])
+
+
+# ------------------------------------------------------------------------------------------------ the loss
+def exact(z, v, i, rest, t, g):
+    """Loss rows and gradient in 64 bits, by the definition: P of every class, one row of everything."""
+    V = z.shape[-1]
+    z, v = z.detach().double(), v.double() / t
+    valid = (i >= 0) & (i < V)
+    v = torch.where(valid, v, torch.full_like(v, -INF))
+    tops = v if rest is None else torch.cat([v, rest.double()[:, None]], 1)
+    some = valid.any(1) & (tops > -INF).any(1)
+    tops = torch.where(some[:, None], tops, torch.zeros_like(tops))
+    pt = torch.softmax(tops, 1)
+    slot = torch.where(valid, i, V).long()
+    P = torch.zeros((z.shape[0], V + 1), device=z.device, dtype=torch.float64).scatter_add(1, slot, pt[:, :v.shape[1]])[:, :V]
+    taken = torch.zeros((z.shape[0], V + 1), device=z.device, dtype=torch.bool).scatter(1, slot, True)[:, :V]
+    lq = torch.log_softmax(torch.where(some[:, None], z, torch.zeros_like(z)) / t, 1)
+    on = P > 0
+    loss = torch.where(on, P * (torch.where(on, P, 1.0).log() - torch.where(on, lq, 0.0)), 0.0).sum(1)
+    dz = lq.exp() - P
+    if rest is not None:
+        pr = pt[:, -1]
+        lt = torch.logsumexp(lq.masked_fill(taken, -INF), 1)
+        on = pr > 0
+        loss = loss + torch.where(on, pr * (torch.where(on, pr, 1.0).log() - torch.where(on, lt, 0.0)), 0.0)
+        cond = torch.where(taken, 0.0, (lq - torch.where(torch.isfinite(lt), lt, 0.0)[:, None]).exp())
+        dz = torch.where(taken, dz, lq.exp() - torch.where(on, pr, 0.0)[:, None] * cond)
+    loss = torch.where(some, loss, 0.0) * t * t
+    dz = torch.where(some[:, None], dz, 0.0) * t * g.double()[:, None]
+    # the parts of a gradient whose roundings count
+    size = torch.where(some[:, None], lq.exp() + P, 0.0) * t * g.double().abs()[:, None]
+    if rest is not None:
+        size = size + torch.where(some[:, None], pr[:, None] * cond, 0.0) * t * g.double().abs()[:, None]
+    return loss, dz, size
+
+
+def check_loss(z, v, i, rest=None, t=1.0, seed=5):
+    V, rows = z.shape[-1], z.numel() // z.shape[-1]
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    g = torch.rand((rows,), device=DEV, generator=gen) * 64 + 1
+    flat = (z.reshape(rows, V), v.reshape(rows, -1), i.reshape(rows, -1), None if rest is None else rest.reshape(rows))
+    loss, dz, size = exact(*flat, t, g)
+    zl = z.detach().requires_grad_(True)
+    row = ops.distill_loss(zl, v, i, rest, t, "none")
+    assert row.dtype == torch.float32 and row.shape == z.shape[:-1]
+    got, = torch.autograd.grad(row, zl, g.view(row.shape))
+    b = 2 * lse_bound(V)
+    diff = (row.detach().reshape(-1).double() - loss).abs()
+    lim = t * t * b + U * loss.abs()
+    assert bool(((diff <= lim) | (row.detach().reshape(-1).double() == loss)).all()), float((diff / lim).max())
+    got = got.reshape(rows, V)
+    half = torch.finfo(z.dtype).eps / 2
+    lim = half * dz.abs() + 2 * b * size + TINY[z.dtype]
+    worst = float(((got.double() - dz).abs() / lim).max())
+    assert worst <= 1.0, f"dz: {worst:.2f} times the bound"
+    for reduction, scale in (("mean", 1.0 / rows), ("sum", 1.0)):
+        total = ops.distill_loss(zl, v, i, rest, t, reduction)
+        assert total.shape == () and abs(float(total.detach()) - float(loss.sum()) * scale) <= scale * (
+            rows * t * t * b + 2 * U * float(loss.abs().sum()))
+        up = torch.tensor(float(rows), device=DEV)
+        gm, = torch.autograd.grad(total, zl, up)
+        lim2 = (half * dz.abs() + 2 * b * size) / g.double()[:, None] * rows * scale + TINY[z.dtype]
+        assert bool(((gm.reshape(rows, V).double() - dz / g.double()[:, None] * rows * scale).abs() <= lim2).all())
+    return row, got
+
+
+def teacher(z, k, t, seed, dtype=None):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    y = 0.8 * z.float() + torch.randn(z.shape, device=DEV, generator=g)
+    return ops.top_logits(y.to(dtype or z.dtype), k, t)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V,k,t", [(1, 1, 1, 1.0), (1, 2, 1, 0.5), (3, 7, 3, 2.0), (2, 64, 64, 1.0), (32, 1000, 5, 1.0),
+                                        (50, 1000, 32, 4.0), (2, 1000, 1000, 1.0), (3, 4097, 1024, 3.0), (9, 50001, 50, 1.0),
+                                        (3, 131072, 64, 2.0), (2, 131071, 1, 8.0), (1, 1 << 20, 16, 1.0)])
+def test_distill_loss_sizes(rows, V, k, t, dtype):
+    z = logits(rows, V, dtype, 6)
+    v, i, r = teacher(z, k, t, 7)
+    check_loss(z, v, i, None, t)
+    check_loss(z, v, i, r, t)
+
+
+@pytest.mark.parametrize("with_rest", [False, True])
+def test_distill_loss_masks(with_rest):
+    rows, V, k, t = 12, 513, 6, 2.0
+    z = logits(rows, V, torch.float32, 8)
+    v, i, r = teacher(z, k, t, 9)
+    i[0] = -1                                     # no entries
+    v[0] = float("nan")
+    i[1, 2:] = -1
+    v[1, 2:] = INF
+    i[2, 0] = V                                   # beyond the classes
+    i[2, 1] = 1 << 40
+    i[3, 3] = i[3, 1]                             # one class twice, one three times
+    i[4, :3] = 11
+    v[5, 1:] = -INF
+    v[6] = -INF
+    r[6] = -INF
+    r[7] = -INF
+    z[8, 100:] = -INF                             # masked classes
+    i[8] = torch.arange(6, device=DEV)
+    z[9, 100:] = torch.finfo(torch.float32).min
+    i[9] = torch.arange(6, device=DEV)
+    z[10, ::3] += 200.0                           # far apart
+    z[0] = float("nan")                           # what stands in a row without entries is not looked at
+    z[6, 5] = INF
+    check_loss(z, v, i, r if with_rest else None, t)
+    check_loss(z, v.half(), i.int(), r if with_rest else None, t)
+
+
+def test_distill_loss_remainder_far_below_the_entries():
+    """Student and teacher put almost everything on the entries: what is left keeps its digits."""
+    z = logits(4, 2048, torch.float32, 10, scale=1.0)
+    i = torch.tensor([[3, 900], [0, 2047], [1, 2], [5, 6]], device=DEV)
+    z.scatter_(1, i, torch.tensor([[30.0, 28.0], [60.0, 61.0], [95.0, 95.0], [20.0, 5.0]], device=DEV))
+    v = torch.tensor([[31.0, 28.0], [60.0, 62.0], [99.0, 95.0], [21.0, 4.0]], device=DEV)
+    r = torch.tensor([8.0, 7.5, 30.0, 8.0], device=DEV)
+    row, dz = check_loss(z, v, i, r)
+    assert bool(torch.isfinite(row).all())
+
+
+def test_distill_loss_nan_and_infinite_rows():
+    z = logits(4, 300, torch.bfloat16, 11)
+    v, i, r = teacher(z, 4, 1.0, 12)
+    z[1, 7] = float("nan")
+    z[2, 7] = INF
+    v[3, 0] = float("nan")
+    zl = z.requires_grad_(True)
+    for rest in (None, r):
+        row = ops.distill_loss(zl, v, i, rest, 1.0, "none")
+        dz, = torch.autograd.grad(row.sum(), zl)
+        assert row.isnan().tolist() == [False, True, True, True]
+        assert not bool(dz[0].isnan().any()) and bool(dz[1].isnan().any()) and bool(dz[2].isnan().any())
+
+
+def test_distill_loss_strides():
+    z = logits(10, 901, torch.float16, 13)
+    v, i, r = teacher(z, 8, 2.0, 14)
+    a = check_loss(z, v, i, r, 2.0)
+    wide = torch.zeros((10, 1000), device=DEV, dtype=torch.float16)
+    wide[:, 3:904] = z
+    vw, iw = torch.zeros((10, 20), device=DEV, dtype=torch.float16), torch.full((10, 20), -1, device=DEV)
+    vw[:, 5:13], iw[:, 5:13] = v, i
+    b = check_loss(wide[:, 3:904], vw[:, 5:13], iw[:, 5:13], r, 2.0)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    c = check_loss(z.view(2, 5, 901), v.view(2, 5, 8), i.view(2, 5, 8), r.view(2, 5), 2.0)
+    assert torch.equal(a[0], c[0].reshape(-1)) and torch.equal(a[1], c[1])
+    check_loss(z.t().contiguous().t(), v.t().contiguous().t(), i.t().contiguous().t(), torch.stack([r, r], 1)[:, 0], 2.0)
+    check_loss(z[:1].expand(10, 901), v[:1].expand(10, 8), i[:1].expand(10, 8), r[:1].expand(10), 2.0)
+
+
+def test_distill_loss_no_rows():
+    z = torch.empty((0, 9), device=DEV, requires_grad=True)
+    loss = ops.distill_loss(z, torch.empty((0, 4), device=DEV), torch.empty((0, 4), device=DEV, dtype=torch.int64), None, 1.0, "sum")
+    loss.backward()
+    assert float(loss) == 0.0 and z.grad.shape == (0, 9)
+
+
+def test_distill_loss_twice_and_on_other_streams():
+    z = logits(40, 5003, torch.bfloat16, 15).requires_grad_(True)
+    v, i, r = teacher(z.detach(), 16, 2.0, 16)
+    loss = ops.distill_loss(z, v, i, r, 2.0)
+    g1, = torch.autograd.grad(loss, z, retain_graph=True)
+    g2, = torch.autograd.grad(loss, z, torch.tensor(3.0, device=DEV), retain_graph=True)
+    keep = g1.clone()
+    g3, = torch.autograd.grad(loss, z)
+    assert torch.equal(g1, g3) and torch.equal(g1, keep)
+    assert float((g2.float() - 3 * g1.float()).abs().max()) <= 3 * 2.0 ** -8 * float(g1.float().abs().max())
+    outs = []
+    for s in [torch.cuda.Stream() for _ in range(2)]:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            l = ops.distill_loss(z, v, i, r, 2.0)
+            outs.append((l, torch.autograd.grad(l, z)[0]))
+        torch.cuda.current_stream().wait_stream(s)
+    for l, g in outs:
+        assert torch.equal(l, loss) and torch.equal(g, g1)
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 1000), (torch.bfloat16, 70001)])
+def test_top_logits_and_distill_loss_captured(dtype, V):
+    zt, zs = logits(6, V, dtype, 17), logits(6, V, dtype, 18).requires_grad_(True)
+
+    def step():
+        v, i, r = ops.top_logits(zt, 20, 2.0)
+        loss = ops.distill_loss(zs, v, i, r, 2.0)
+        return v, i, r, loss, torch.autograd.grad(loss, zs)[0]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(4):
+        with torch.no_grad():
+            zt.copy_(logits(6, V, dtype, 30 + k))
+            zs.copy_(logits(6, V, dtype, 40 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
