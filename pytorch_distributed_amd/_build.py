@@ -19,6 +19,7 @@ from __future__ import annotations
 import concurrent.futures as cf
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -56,6 +57,18 @@ def _run(cmd) -> None:
         raise RuntimeError("build step failed:\n  %s\n%s\n%s" % (" ".join(map(str, cmd)), r.stdout, r.stderr))
 
 
+def _included(src: Path) -> list:
+    """The headers of its own folder that a source includes, directly or through one another."""
+    found, todo = {}, [src]
+    while todo:
+        for name in re.findall(r'^\s*#include\s+"([^"]+)"', todo.pop().read_text(), re.M):
+            h = src.parent / name
+            if h.exists() and h not in found:
+                found[h] = True
+                todo.append(h)
+    return list(found)
+
+
 def _needs(target: Path, stamp: str) -> bool:
     sf = target.with_suffix(target.suffix + ".stamp")
     return not (target.exists() and sf.exists() and sf.read_text() == stamp)
@@ -75,11 +88,9 @@ def build_kernels(force: bool = False, jobs: int | None = None, verbose: bool = 
     LIB.mkdir(exist_ok=True)
     OBJ.mkdir(exist_ok=True)
     jobs = jobs or min(8, os.cpu_count() or 4, int(os.environ.get("MAX_JOBS", "8")))
-    hstamp = _stamp(hdrs) + flags
-
     def one(src: Path) -> Path:
         obj = OBJ / (src.stem + ".o")
-        st = _stamp([src]) + hstamp
+        st = _stamp([src] + _included(src)) + flags
         if force or _needs(obj, st):
             if verbose:
                 print("[pda build] hipcc", src.name, flush=True)

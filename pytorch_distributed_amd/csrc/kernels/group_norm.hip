@@ -1,34 +1,19 @@
-// Group norm with an optional residual and activation, channels last: x [N][S][C], C = G groups of D channels, m = S*D.
-//   mu, var over the m elements of a (sample, group); r = 1/sqrt(var + eps); xh = (x - mu) r
-//   z = xh*gamma_c + beta_c + res;  out = act(z), act = identity | max(z, 0) | min(max(z, 0), cap) | z*sigmoid(z)
-// Backward with g = dout*act'(z) (z is computed again from x and res, nothing of it is kept):
-//   dres = g,  dbeta_c = sum_{n,s} g,  dgamma_c = sum_{n,s} g xh
-//   A = sum_{group} gamma g, B = sum_{group} gamma g xh;  dx = r (gamma g - (A + xh B)/m)
+// Group norm with an optional residual and activation, channels last: x [N][S][C], C = G groups of D channels.  The formulas
+// are those of group_norm.h.
 //
 // Statistics: a thread takes its rows in batches of four, relative to the first row of its chunk (a mean far from zero
 // costs no digits), forms each batch's mean and centred squares in fp32 and adds batches up in fp64; (sample, group)
-// totals are fp64 and kept as pairs {mu, r}.  16-bit inputs lose nothing in a batch, so their statistics are good to far
-// below fp32: the side of an activation's border on which a value lies can be decided from them (gn_grad).  The element
-// passes take mu as an fp32 pair (hi subtracted from x, lo folded into the shift).
+// totals are fp64 and kept as pairs {mu, r}.  16-bit inputs lose next to nothing in a batch, so their statistics are good
+// to far below fp32, and the side of an activation's border on which a value lies is decided from them in fp64.
 //
 // Memory-bound throughout: the work is split over (sample, row chunk), a thread owns one vector of channels and walks
 // rows, so the per-channel coefficients stay in registers.  No atomics: results repeat bit for bit.
-#include "common.h"
+#include "group_norm.h"
 
 #include <initializer_list>
+#include <math.h>
 
 namespace {
-
-enum GnAct : int { GN_NONE = 0, GN_RELU = 1, GN_CAP = 2, GN_SILU = 3 };
-
-struct GnStat { double mean, rstd; };
-
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) GnVec { T v[VEC]; };
-
-template <typename T, int VEC>
-__device__ __forceinline__ GnVec<T, VEC> gn_ld(const T* p) { return *reinterpret_cast<const GnVec<T, VEC>*>(p); }
-template <typename T, int VEC>
-__device__ __forceinline__ void gn_st(T* p, const GnVec<T, VEC>& v) { *reinterpret_cast<GnVec<T, VEC>*>(p) = v; }
 
 // Where a block's threads stand: VT vectors of channels side by side, RS rows at a time (threads beyond VT*RS idle).
 struct GnGeom {
@@ -123,12 +108,6 @@ gn_partial_kernel(const T* __restrict__ x, long long S, int C, int chunks, GnSum
   }
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
 // One wave per (sample, group): chunks x D sums -> {mu, r} in fp64.
 template <typename T>
 __global__ void __launch_bounds__(64)
@@ -163,86 +142,59 @@ gn_finalize_kernel(const T* __restrict__ x, const GnSums* __restrict__ part, lon
   if (threadIdx.x == 0) stats[blockIdx.x] = GnStat{mean, 1.0 / sqrt(q / m + eps)};
 }
 
-// Coefficients of one channel: z = (x - mh)*sc + sh (+ res), xh = (x - mh - ml)*r
-struct GnCoef { float mh, ml, r, sc, sh; };
-__device__ __forceinline__ GnCoef gn_coef(const GnStat& st, float gamma, float beta) {
-  GnCoef k;
-  k.mh = (float)st.mean;
-  k.ml = (float)(st.mean - (double)k.mh);
-  k.r = (float)st.rstd;
-  k.sc = (float)(st.rstd * (double)gamma);
-  k.sh = beta - k.ml * k.sc;
-  return k;
-}
-
-__device__ __forceinline__ float gn_act(float z, int act, float cap) {
-  if (act == GN_SILU) return z / (1.f + __expf(-z));
-  if (act != GN_NONE) z = z < 0.f ? 0.f : z;      // a NaN stays one
-  if (act == GN_CAP) z = z > cap ? cap : z;
-  return z;
-}
-
-// g = dy * act'(z).  A z within rounding of a border of the activation is computed again in fp64 from the fp64
-// statistics: on which side it lies decides over the whole gradient of the element.
-__device__ __forceinline__ float gn_grad(float dy, float x, float res, const GnCoef& k, int act, float cap,
-                                         const GnStat* st, const float* gamma, const float* beta, int c) {
-  if (act == GN_NONE) return dy;
-  const float t = (x - k.mh) * k.sc;
-  const float z = t + k.sh + res;
-  if (act == GN_SILU) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return dy * (s * (1.f + z * (1.f - s)));
-  }
-  const float tol = 1e-6f * (fabsf(t) + fabsf(k.sh) + fabsf(res));
-  bool on = z > 0.f && (act != GN_CAP || z < cap);
-  if (fabsf(z) < tol || (act == GN_CAP && fabsf(z - cap) < tol)) {
-    const double zd = ((double)x - st->mean) * st->rstd * (gamma ? (double)gamma[c] : 1.0) +
-                      (beta ? (double)beta[c] : 0.0) + (double)res;
-    on = zd > 0.0 && (act != GN_CAP || zd < (double)cap);
-  }
-  return on ? dy : 0.f;
-}
-
-template <typename T, int VEC>
+template <typename T, int VEC, bool UG, int ACT>
 __global__ void __launch_bounds__(256)
 gn_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ out, const float* __restrict__ gamma,
                 const float* __restrict__ beta, const GnStat* __restrict__ stats, long long S, int C, int G, int chunks,
-                int act, float cap) {
+                float cap) {
+  constexpr int U = 2;  // rows in flight
   const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
   const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
   const int vpr = C / VEC, D = C / G;
   const GnGeom g(vpr);
   if (g.rl >= g.RS) return;
   for (int vec = g.col; vec < vpr; vec += g.VT) {
-    GnCoef k[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int c = vec * VEC + e;
-      k[e] = gn_coef(stats[(long long)n * G + c / D], gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
-    }
+    GnCoef<VEC, UG> k;
+    k.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
     const long long base = (long long)n * S * C + (long long)vec * VEC;
-#pragma unroll 2
-    for (long long r = r0 + g.rl; r < r1; r += g.RS) {
-      const long long o = base + r * C;
-      GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), w;
-      if (res) w = gn_ld<T, VEC>(res + o);
+    const auto row = [&](GnVec<T, VEC>& v, const GnVec<T, VEC>& w) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float z = (ElemTraits<T>::to_f32(v.v[e]) - k[e].mh) * k[e].sc + k[e].sh;
+        float z = (ElemTraits<T>::to_f32(v.v[e]) - k.mh[UG ? 0 : e]) * k.sc[e] + k.sh[e];
         if (res) z += ElemTraits<T>::to_f32(w.v[e]);
-        v.v[e] = ElemTraits<T>::from_f32(gn_act(z, act, cap));
+        v.v[e] = ElemTraits<T>::from_f32(gn_act<ACT>(z, cap));
       }
-      gn_st<T, VEC>(out + o, v);
+    };
+    long long r = r0 + g.rl;
+    for (; r + (U - 1) * g.RS < r1; r += U * g.RS) {
+      GnVec<T, VEC> v[U], w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        v[u] = gn_ld<T, VEC>(x + base + (r + u * g.RS) * C);
+        if (res) w[u] = gn_ld<T, VEC>(res + base + (r + u * g.RS) * C);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        row(v[u], w[u]);
+        gn_st<T, VEC>(out + base + (r + u * g.RS) * C, v[u]);
+      }
+    }
+    for (; r < r1; r += g.RS) {
+      GnVec<T, VEC> v = gn_ld<T, VEC>(x + base + r * C), w;
+      if (res) w = gn_ld<T, VEC>(res + base + r * C);
+      row(v, w);
+      gn_st<T, VEC>(out + base + r * C, v);
     }
   }
 }
 
 // Per-channel {sum g, sum g xh} of one row chunk of one sample -> part[n][chunk][c].
-template <typename T, int VEC>
+template <typename T, int VEC, bool UG, int ACT>
 __global__ void __launch_bounds__(256)
 gn_bwd_partial_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout,
                       const float* __restrict__ gamma, const float* __restrict__ beta, const GnStat* __restrict__ stats,
-                      long long S, int C, int G, int chunks, int act, float cap, float2* __restrict__ part) {
+                      long long S, int C, int G, int chunks, double cap, float2* __restrict__ part) {
+  constexpr int U = 2;
   __shared__ float sa[256 * VEC], sb[256 * VEC];
   const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
   const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
@@ -255,29 +207,45 @@ gn_bwd_partial_kernel(const T* __restrict__ x, const T* __restrict__ res, const 
 #pragma unroll
     for (int e = 0; e < VEC; ++e) a[e] = b[e] = 0.f;
     if (active) {
-      GnCoef k[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int c = vec * VEC + e;
-        k[e] = gn_coef(stats[(long long)n * G + c / D], gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
-      }
+      GnCoef<VEC, UG> k;
+      typename GnBorderOf<ACT, VEC>::type bd;
+      k.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
+      bd.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
       const long long base = (long long)n * S * C + (long long)vec * VEC;
-#pragma unroll 2
-      for (long long r = r0 + g.rl; r < r1; r += g.RS) {
+      const bool wr = ACT != GN_NONE && res;
+      const auto row = [&](const GnVec<T, VEC>& v, const GnVec<T, VEC>& d, const GnVec<T, VEC>& w) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float xf = ElemTraits<T>::to_f32(v.v[e]), t = xf - k.mh[UG ? 0 : e];
+          const float gr = gn_grad<ACT, VEC>(ElemTraits<T>::to_f32(d.v[e]), xf, t, wr ? ElemTraits<T>::to_f32(w.v[e]) : 0.f,
+                                             k.sc[e], k.sh[e], bd, e, cap);
+          a[e] += gr;
+          b[e] += gr * t;
+        }
+      };
+      long long r = r0 + g.rl;
+      for (; r + (U - 1) * g.RS < r1; r += U * g.RS) {
+        GnVec<T, VEC> v[U], d[U], w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const long long o = base + (r + u * g.RS) * C;
+          v[u] = gn_ld<T, VEC>(x + o);
+          d[u] = gn_ld<T, VEC>(dout + o);
+          if (wr) w[u] = gn_ld<T, VEC>(res + o);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) row(v[u], d[u], w[u]);
+      }
+      for (; r < r1; r += g.RS) {
         const long long o = base + r * C;
         const GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), d = gn_ld<T, VEC>(dout + o);
         GnVec<T, VEC> w;
-        if (res) w = gn_ld<T, VEC>(res + o);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const int c = vec * VEC + e;
-          const float xf = ElemTraits<T>::to_f32(v.v[e]);
-          const float gr = gn_grad(ElemTraits<T>::to_f32(d.v[e]), xf, res ? ElemTraits<T>::to_f32(w.v[e]) : 0.f, k[e], act,
-                                   cap, stats + (long long)n * G + c / D, gamma, beta, c);
-          a[e] += gr;
-          b[e] += gr * ((xf - k[e].mh - k[e].ml) * k[e].r);
-        }
+        if (wr) w = gn_ld<T, VEC>(res + o);
+        row(v, d, w);
       }
+      // sum g (x - mh) -> sum g xh
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) b[e] = (b[e] - k.ml[UG ? 0 : e] * a[e]) * k.r[UG ? 0 : e];
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -368,45 +336,66 @@ gn_params_kernel(const float2* __restrict__ part, long long rows, int C, float* 
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool UG, int ACT>
 __global__ void __launch_bounds__(256)
 gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout, T* __restrict__ dx,
                     T* __restrict__ dres, const float* __restrict__ gamma, const float* __restrict__ beta,
                     const GnStat* __restrict__ stats, const float2* __restrict__ ab, long long S, int C, int G, int chunks,
-                    int act, float cap) {
+                    double cap) {
+  constexpr int U = 2;
   const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
   const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
   const int vpr = C / VEC, D = C / G;
   const GnGeom g(vpr);
   if (g.rl >= g.RS) return;
   for (int vec = g.col; vec < vpr; vec += g.VT) {
-    GnCoef k[VEC];
-    float pa[VEC], pb[VEC];
+    GnCoef<VEC, UG> k;
+    typename GnBorderOf<ACT, VEC>::type bd;
+    k.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
+    bd.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
+    float pa[k.NG], pb[k.NG];  // dx = g*sc + pa + (x - mh)*pb
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int c = vec * VEC + e;
-      const long long i = (long long)n * G + c / D;
-      k[e] = gn_coef(stats[i], gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
-      const float2 v = ab[i];
-      pa[e] = -v.x * k[e].r;
-      pb[e] = -v.y * k[e].r;
+    for (int i = 0; i < k.NG; ++i) {
+      const float2 v = ab[(long long)n * G + (vec * VEC + i) / D];
+      pb[i] = -v.y * k.r[i] * k.r[i];
+      pa[i] = -v.x * k.r[i] - k.ml[i] * pb[i];
     }
     const long long base = (long long)n * S * C + (long long)vec * VEC;
-#pragma unroll 2
-    for (long long r = r0 + g.rl; r < r1; r += g.RS) {
-      const long long o = base + r * C;
-      GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), d = gn_ld<T, VEC>(dout + o), w;
-      if (res) w = gn_ld<T, VEC>(res + o);
+    const bool wr = ACT != GN_NONE && res;
+    const auto row = [&](GnVec<T, VEC>& v, GnVec<T, VEC>& d, const GnVec<T, VEC>& w) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const int c = vec * VEC + e;
-        const float xf = ElemTraits<T>::to_f32(v.v[e]);
-        const float gr = gn_grad(ElemTraits<T>::to_f32(d.v[e]), xf, res ? ElemTraits<T>::to_f32(w.v[e]) : 0.f, k[e], act, cap,
-                                 stats + (long long)n * G + c / D, gamma, beta, c);
-        const float xh = (xf - k[e].mh - k[e].ml) * k[e].r;
-        v.v[e] = ElemTraits<T>::from_f32(gr * k[e].sc + (pa[e] + xh * pb[e]));
+        const int i = UG ? 0 : e;
+        const float xf = ElemTraits<T>::to_f32(v.v[e]), t = xf - k.mh[i];
+        const float gr = gn_grad<ACT, VEC>(ElemTraits<T>::to_f32(d.v[e]), xf, t, wr ? ElemTraits<T>::to_f32(w.v[e]) : 0.f,
+                                           k.sc[e], k.sh[e], bd, e, cap);
+        v.v[e] = ElemTraits<T>::from_f32(gr * k.sc[e] + (t * pb[i] + pa[i]));
         d.v[e] = ElemTraits<T>::from_f32(gr);
       }
+    };
+    long long r = r0 + g.rl;
+    for (; r + (U - 1) * g.RS < r1; r += U * g.RS) {
+      GnVec<T, VEC> v[U], d[U], w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long o = base + (r + u * g.RS) * C;
+        v[u] = gn_ld<T, VEC>(x + o);
+        d[u] = gn_ld<T, VEC>(dout + o);
+        if (wr) w[u] = gn_ld<T, VEC>(res + o);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long o = base + (r + u * g.RS) * C;
+        row(v[u], d[u], w[u]);
+        gn_st<T, VEC>(dx + o, v[u]);
+        if (dres) gn_st<T, VEC>(dres + o, d[u]);
+      }
+    }
+    for (; r < r1; r += g.RS) {
+      const long long o = base + r * C;
+      GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), d = gn_ld<T, VEC>(dout + o), w;
+      if (wr) w = gn_ld<T, VEC>(res + o);
+      row(v, d, w);
       gn_st<T, VEC>(dx + o, v);
       if (dres) gn_st<T, VEC>(dres + o, d);
     }
@@ -424,24 +413,41 @@ int gn_vec(int C, int esize, std::initializer_list<const void*> ptrs) {
   return 1;
 }
 
+// act: 0 none, 1 ReLU, 2 ReLU clipped at cap, 3 SiLU (the codes of the Python side)
 bool gn_args_ok(long long N, long long S, int C, int G, int chunks, int act) {
-  return N > 0 && S > 0 && C > 0 && G > 0 && C % G == 0 && chunks > 0 && chunks <= S && act >= GN_NONE && act <= GN_SILU &&
+  return N > 0 && S > 0 && C > 0 && G > 0 && C % G == 0 && chunks > 0 && chunks <= S && act >= 0 && act <= 3 &&
          N * chunks < (1ll << 31) && N * G < (1ll << 31);
+}
+int gn_act_class(int act, float& cap) {
+  if (act == 1) cap = INFINITY;
+  return act == 0 ? GN_NONE : act == 3 ? GN_SILU : GN_CAP;
 }
 
 }  // namespace
 
 #define GN_VEC_CASE(T, V, ...) case V: { constexpr int VEC = V; typedef T E; __VA_ARGS__; } break;
-#define GN_DISPATCH(dtype, vec, ...)                                                                     \
-  switch (dtype) {                                                                                        \
-    case PDA_F32: switch (vec) { GN_VEC_CASE(float, 4, __VA_ARGS__) GN_VEC_CASE(float, 2, __VA_ARGS__)                  \
-                                 default: { constexpr int VEC = 1; typedef float E; __VA_ARGS__; } } break;      \
-    case PDA_F16: switch (vec) { GN_VEC_CASE(f16, 8, __VA_ARGS__) GN_VEC_CASE(f16, 4, __VA_ARGS__) GN_VEC_CASE(f16, 2, __VA_ARGS__) \
-                                 default: { constexpr int VEC = 1; typedef f16 E; __VA_ARGS__; } } break;        \
-    case PDA_BF16: switch (vec) { GN_VEC_CASE(bf16, 8, __VA_ARGS__) GN_VEC_CASE(bf16, 4, __VA_ARGS__) GN_VEC_CASE(bf16, 2, __VA_ARGS__) \
-                                  default: { constexpr int VEC = 1; typedef bf16 E; __VA_ARGS__; } } break;      \
-    default: return -6;                                                                                   \
+#define GN_DISPATCH(dtype, vec, ...)                                                                                  \
+  switch (dtype) {                                                                                                    \
+    case PDA_F32: switch (vec) { GN_VEC_CASE(float, 4, __VA_ARGS__) GN_VEC_CASE(float, 2, __VA_ARGS__)                \
+                                 default: { constexpr int VEC = 1; typedef float E; __VA_ARGS__; } } break;           \
+    case PDA_F16: switch (vec) { GN_VEC_CASE(f16, 8, __VA_ARGS__) GN_VEC_CASE(f16, 4, __VA_ARGS__)                    \
+                                 GN_VEC_CASE(f16, 2, __VA_ARGS__)                                                     \
+                                 default: { constexpr int VEC = 1; typedef f16 E; __VA_ARGS__; } } break;             \
+    case PDA_BF16: switch (vec) { GN_VEC_CASE(bf16, 8, __VA_ARGS__) GN_VEC_CASE(bf16, 4, __VA_ARGS__)                 \
+                                  GN_VEC_CASE(bf16, 2, __VA_ARGS__)                                                   \
+                                  default: { constexpr int VEC = 1; typedef bf16 E; __VA_ARGS__; } } break;           \
+    default: return -6;                                                                                               \
   }
+// ... and over the activation class and whether a vector of channels lies in one group
+#define GN_DISPATCH_ACT(act, ug, ...)                                                          \
+  switch (act) {                                                                               \
+    case GN_NONE: { constexpr int ACT = GN_NONE; GN_UG(ug, __VA_ARGS__) } break;               \
+    case GN_CAP: { constexpr int ACT = GN_CAP; GN_UG(ug, __VA_ARGS__) } break;                 \
+    default: { constexpr int ACT = GN_SILU; GN_UG(ug, __VA_ARGS__) } break;                    \
+  }
+#define GN_UG(ug, ...)                                                                                        \
+  if (ug && VEC * sizeof(E) == 16) { constexpr bool UG = VEC * sizeof(E) == 16; __VA_ARGS__; }                \
+  else { constexpr bool UG = false; __VA_ARGS__; }
 
 // Row chunks per sample: about 2048 blocks over the chip, at least 8 rows for each thread of a block.
 PDA_EXPORT int pda_group_norm_chunks(int dtype, long long N, long long S, int C) {
@@ -464,9 +470,10 @@ PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x, const void* res, voi
                                              chunks, (GnSums*)part));
   GN_DISPATCH(dtype, 1, hipLaunchKernelGGL((gn_finalize_kernel<E>), dim3((int)(N * G)), dim3(64), 0, st, (const E*)x,
                                            (const GnSums*)part, S, C, G, chunks, eps, (GnStat*)stats));
-  GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_apply_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x,
-                                             (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, act,
-                                             cap));
+  const int cls = gn_act_class(act, cap);
+  const bool ug = (C / G) % vec == 0;
+  GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_apply_kernel<E, VEC, UG, ACT>), dim3(blocks), dim3(256),
+              0, st, (const E*)x, (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, cap)));
   return pda_check_launch();
 }
 
@@ -478,17 +485,19 @@ PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x, const void* res, con
   if (!gn_args_ok(N, S, C, G, chunks, act) || (dres && !dx)) return -1;
   const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, dout, dx, dres});
   const int blocks = (int)(N * chunks);
-  GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_bwd_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x,
-                                             (const E*)res, (const E*)dout, gamma, beta, (const GnStat*)stats, S, C, G, chunks,
-                                             act, cap, (float2*)part));
+  const int cls = gn_act_class(act, cap);
+  const bool ug = (C / G) % vec == 0;
+  GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_bwd_partial_kernel<E, VEC, UG, ACT>), dim3(blocks),
+              dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, gamma, beta, (const GnStat*)stats, S, C, G, chunks,
+              (double)cap, (float2*)part)));
   hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const float2*)part, gamma, S, C, G, chunks,
                      (float2*)ab);
   if (dgamma)
     hipLaunchKernelGGL(gn_params_kernel, dim3((C + 3) / 4), dim3(1024), 0, st, (const float2*)part, N * chunks, C, dgamma,
                        dbeta);
   if (dx)
-    GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_bwd_apply_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x,
-                                               (const E*)res, (const E*)dout, (E*)dx, (E*)dres, gamma, beta,
-                                               (const GnStat*)stats, (const float2*)ab, S, C, G, chunks, act, cap));
+    GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_bwd_apply_kernel<E, VEC, UG, ACT>), dim3(blocks),
+                dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, (E*)dx, (E*)dres, gamma, beta,
+                (const GnStat*)stats, (const float2*)ab, S, C, G, chunks, (double)cap)));
   return pda_check_launch();
 }
