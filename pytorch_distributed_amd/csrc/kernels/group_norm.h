@@ -11,51 +11,67 @@ enum GnAct : int { GN_NONE = 0, GN_CAP = 1, GN_SILU = 2 };
 
 struct GnStat { double mean, rstd; };
 
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) GnVec { T v[VEC]; };
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) GnVec {
+  T v[VEC];
+  __device__ __forceinline__ float f(int e) const { return ElemTraits<T>::to_f32(v[e]); }
+};
+
+// 16 bytes as four registers.  A vector that lives across branches and barriers is kept like this: as elements the
+// compiler unpacks it at once, into twice the registers.
+template <typename T> struct GnRaw {
+  u32x4 u;
+  __device__ __forceinline__ float f(int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u[e]);
+    else {
+      const unsigned short h = (unsigned short)(e & 1 ? u[e >> 1] >> 16 : u[e >> 1]);
+      return ElemTraits<T>::to_f32(__builtin_bit_cast(T, h));
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[16 / sizeof(T)]) {
+    GnVec<T, 16 / sizeof(T)> v;
+#pragma unroll
+    for (int e = 0; e < (int)(16 / sizeof(T)); ++e) v.v[e] = ElemTraits<T>::from_f32(x[e]);
+    u = __builtin_bit_cast(u32x4, v);
+  }
+};
+template <typename T> __device__ __forceinline__ GnRaw<T> gn_ld_raw(const T* p) {
+  return GnRaw<T>{*reinterpret_cast<const u32x4*>(p)};
+}
+template <typename T> __device__ __forceinline__ void gn_st_raw(T* p, const GnRaw<T>& v) { *reinterpret_cast<u32x4*>(p) = v.u; }
 
 template <typename T, int VEC>
 __device__ __forceinline__ GnVec<T, VEC> gn_ld(const T* p) { return *reinterpret_cast<const GnVec<T, VEC>*>(p); }
 template <typename T, int VEC>
 __device__ __forceinline__ void gn_st(T* p, const GnVec<T, VEC>& v) { *reinterpret_cast<GnVec<T, VEC>*>(p) = v; }
 
-// Coefficients of the VEC channels of one thread.  UG: they lie in one group, whose mean and deviation are held once.
-//   forward: z = (x - mh)*sc + sh;  the mean is the fp32 pair (mh, ml), ml folded into sh
+// Coefficients of the VEC channels of one thread: z = (x - mh)*sc + sh.  The mean is the fp32 pair (mh, ml), ml folded into
+// sh.  UG: the channels lie in one group, whose mean is held once.
 template <int VEC, bool UG> struct GnCoef {
   static constexpr int NG = UG ? 1 : VEC;
-  float mh[NG], ml[NG], r[NG], sc[VEC], sh[VEC];
+  float mh[NG], sc[VEC], sh[VEC];
   __device__ __forceinline__ void load(const GnStat* st /* of this sample */, const float* gamma, const float* beta, int c0,
                                        int D) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int k = UG ? 0 : e;
       const GnStat s = st[(UG ? c0 : c0 + e) / D];
-      mh[k] = (float)s.mean;
-      ml[k] = (float)(s.mean - (double)mh[k]);
-      r[k] = (float)s.rstd;
+      const float m = (float)s.mean;
+      mh[UG ? 0 : e] = m;
       sc[e] = (float)(s.rstd * (double)(gamma ? gamma[c0 + e] : 1.f));
-      sh[e] = (beta ? beta[c0 + e] : 0.f) - ml[k] * sc[e];
+      sh[e] = (beta ? beta[c0 + e] : 0.f) - (float)(s.mean - (double)m) * sc[e];
     }
   }
 };
 
-// The pre-activation in fp64, z = x*sc + sh: on which side of an activation's border a value lies decides over the whole
-// gradient of the element, and fp64 multiply-adds cost what fp32 ones do.
-template <int VEC> struct GnBorder {
-  double sc[VEC], sh[VEC];
-  __device__ __forceinline__ void load(const GnStat* st, const float* gamma, const float* beta, int c0, int D) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const GnStat s = st[(c0 + e) / D];
-      sc[e] = s.rstd * (double)(gamma ? gamma[c0 + e] : 1.f);
-      sh[e] = (double)(beta ? beta[c0 + e] : 0.f) - s.mean * sc[e];
-    }
-  }
-};
-struct GnNoBorder {
-  __device__ __forceinline__ void load(const GnStat*, const float*, const float*, int, int) {}
-};
-template <int ACT, int VEC> struct GnBorderOf { typedef GnNoBorder type; };
-template <int VEC> struct GnBorderOf<GN_CAP, VEC> { typedef GnBorder<VEC> type; };
+// sum g (x - mh) of a channel -> sum g xh
+__device__ __forceinline__ float gn_centre(float gt, float g, const GnStat& s) {
+  return (gt - (float)(s.mean - (double)(float)s.mean) * g) * (float)s.rstd;
+}
+// dx = g*sc + pa + (x - mh)*pb, from A/m and B/m
+__device__ __forceinline__ void gn_dx_coefs(float A, float B, const GnStat& s, float& pa, float& pb) {
+  const float r = (float)s.rstd;
+  pb = -B * r * r;
+  pa = -A * r - (float)(s.mean - (double)(float)s.mean) * pb;
+}
 
 __device__ __forceinline__ float gn_sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
@@ -70,20 +86,71 @@ template <int ACT> __device__ __forceinline__ float gn_act(float z, float cap) {
   return z;
 }
 
-// g of one element; x as stored, t = x - mh.
-template <int ACT, int VEC, typename B>
-__device__ __forceinline__ float gn_grad(float dy, float x, float t, float res, float sc, float sh, const B& b, int e,
-                                         double cap) {
-  if constexpr (ACT == GN_NONE) return dy;
-  if constexpr (ACT == GN_SILU) {
-    const float z = t * sc + sh + res, s = gn_sigmoid(z);
-    return dy * (s * (1.f + z * (1.f - s)));
+// Which of a vector's pre-activations lie between the borders 0 and cap, in fp64 from the fp64 statistics.
+template <typename T, int VEC>
+__device__ __forceinline__ unsigned gn_inside(const T* x, const T* res, const GnStat* st, const float* gamma, const float* beta,
+                                              int c0, int D, float cap) {
+  unsigned on = 0;
+#pragma unroll 1
+  for (int e = 0; e < VEC; ++e) {
+    const GnStat s = st[(c0 + e) / D];
+    const double z = ((double)ElemTraits<T>::to_f32(x[e]) - s.mean) * s.rstd * (gamma ? (double)gamma[c0 + e] : 1.0) +
+                     (beta ? (double)beta[c0 + e] : 0.0) + (res ? (double)ElemTraits<T>::to_f32(res[e]) : 0.0);
+    on |= z > 0.0 && z < (double)cap ? 1u << e : 0u;
   }
+  return on;
+}
+
+// act'(z) of the clipped ReLU for a vector: one bit an element, and whether one lies so near a border of the activation (16
+// fp32 roundings of its parts) that gn_inside has to decide: on which side it lies decides over its whole gradient.
+template <typename V, int VEC, bool UG>
+__device__ __forceinline__ unsigned gn_bits(const V& v, const V& w, bool wr, const GnCoef<VEC, UG>& k, float cap, bool& near) {
+  unsigned on = 0;
+  near = false;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const float t = (v.f(e) - k.mh[UG ? 0 : e]) * k.sc[e];
+    float z = t + k.sh[e];
+    if (wr) z += w.f(e);
+    // (at 0 a residual is as large as t + sh; at the cap it is at most that and the cap)
+    const float a = fabsf(t) + fabsf(k.sh[e]);
+    near |= fabsf(z) < 1e-6f * a || fabsf(z - cap) < 1e-6f * (a + cap);
+    on |= z > 0.f && z < cap ? 1u << e : 0u;
+  }
+  return on;
+}
+template <typename V, int VEC, bool UG>
+__device__ __forceinline__ float gn_silu_slope(const V& v, const V& w, bool wr, const GnCoef<VEC, UG>& k, int e) {
+  float z = (v.f(e) - k.mh[UG ? 0 : e]) * k.sc[e] + k.sh[e];
+  if (wr) z += w.f(e);
+  const float s = gn_sigmoid(z);
+  return s * (1.f + z * (1.f - s));
+}
+
+// g = dout*act'(z) of a vector; x and res where they stand, c0 the channel of x[0].
+template <int ACT, typename T, int VEC, bool UG>
+__device__ __forceinline__ void gn_grads(float (&g)[VEC], const GnVec<T, VEC>& d, const GnVec<T, VEC>& v, const GnVec<T, VEC>& w,
+                                         bool wr, const GnCoef<VEC, UG>& k, const T* x, const T* res, const GnStat* st,
+                                         const float* gamma, const float* beta, int c0, int D, float cap) {
+  unsigned on = 0;
   if constexpr (ACT == GN_CAP) {
-    const double z = (double)x * b.sc[e] + b.sh[e] + (double)res;
-    return z > 0.0 && z < cap ? dy : 0.f;
+    bool near;
+    on = gn_bits(v, w, wr, k, cap, near);
+    if (near) on = gn_inside<T, VEC>(x, wr ? res : nullptr, st, gamma, beta, c0, D, cap);
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const float dy = ElemTraits<T>::to_f32(d.v[e]);
+    if constexpr (ACT == GN_NONE) g[e] = dy;
+    if constexpr (ACT == GN_CAP) g[e] = (on >> e) & 1u ? dy : 0.f;
+    if constexpr (ACT == GN_SILU) g[e] = dy * gn_silu_slope(v, w, wr, k, e);
   }
 }
+
+// Makes the compiler take a vector (or an offset) as new: what was computed from it - its elements in fp32, the addresses of
+// a pass - is not kept in registers for the next pass.
+template <typename T> __device__ __forceinline__ void gn_renew(GnRaw<T>& v) { asm volatile("" : "+v"(v.u)); }
+__device__ __forceinline__ void gn_renew(unsigned& v) { asm volatile("" : "+v"(v)); }
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll

@@ -4,11 +4,11 @@
 // Statistics: a thread takes its rows in batches of four, relative to the first row of its chunk (a mean far from zero
 // costs no digits), forms each batch's mean and centred squares in fp32 and adds batches up in fp64; (sample, group)
 // totals are fp64 and kept as pairs {mu, r}.  16-bit inputs lose next to nothing in a batch, so their statistics are good
-// to far below fp32, and the side of an activation's border on which a value lies is decided from them in fp64.
+// to far below fp32; a value next to an activation's border is placed by them in fp64.
 //
 // Memory-bound throughout: the work is split over (sample, row chunk), a thread owns one vector of channels and walks
 // rows, so the per-channel coefficients stay in registers.  No atomics: results repeat bit for bit.
-#include "group_norm.h"
+#include "group_norm_resident.h"
 
 #include <initializer_list>
 #include <math.h>
@@ -193,7 +193,7 @@ template <typename T, int VEC, bool UG, int ACT>
 __global__ void __launch_bounds__(256)
 gn_bwd_partial_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout,
                       const float* __restrict__ gamma, const float* __restrict__ beta, const GnStat* __restrict__ stats,
-                      long long S, int C, int G, int chunks, double cap, float2* __restrict__ part) {
+                      long long S, int C, int G, int chunks, float cap, float2* __restrict__ part) {
   constexpr int U = 2;
   __shared__ float sa[256 * VEC], sb[256 * VEC];
   const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
@@ -208,19 +208,17 @@ gn_bwd_partial_kernel(const T* __restrict__ x, const T* __restrict__ res, const 
     for (int e = 0; e < VEC; ++e) a[e] = b[e] = 0.f;
     if (active) {
       GnCoef<VEC, UG> k;
-      typename GnBorderOf<ACT, VEC>::type bd;
-      k.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
-      bd.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
+      const GnStat* stn = stats + (long long)n * G;
+      k.load(stn, gamma, beta, vec * VEC, D);
       const long long base = (long long)n * S * C + (long long)vec * VEC;
       const bool wr = ACT != GN_NONE && res;
-      const auto row = [&](const GnVec<T, VEC>& v, const GnVec<T, VEC>& d, const GnVec<T, VEC>& w) {
+      const auto row = [&](const GnVec<T, VEC>& v, const GnVec<T, VEC>& d, const GnVec<T, VEC>& w, long long o) {
+        float gr[VEC];
+        gn_grads<ACT>(gr, d, v, w, wr, k, x + o, res + o, stn, gamma, beta, vec * VEC, D, cap);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const float xf = ElemTraits<T>::to_f32(v.v[e]), t = xf - k.mh[UG ? 0 : e];
-          const float gr = gn_grad<ACT, VEC>(ElemTraits<T>::to_f32(d.v[e]), xf, t, wr ? ElemTraits<T>::to_f32(w.v[e]) : 0.f,
-                                             k.sc[e], k.sh[e], bd, e, cap);
-          a[e] += gr;
-          b[e] += gr * t;
+          a[e] += gr[e];
+          b[e] += gr[e] * (ElemTraits<T>::to_f32(v.v[e]) - k.mh[UG ? 0 : e]);
         }
       };
       long long r = r0 + g.rl;
@@ -234,18 +232,17 @@ gn_bwd_partial_kernel(const T* __restrict__ x, const T* __restrict__ res, const 
           if (wr) w[u] = gn_ld<T, VEC>(res + o);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) row(v[u], d[u], w[u]);
+        for (int u = 0; u < U; ++u) row(v[u], d[u], w[u], base + (r + u * g.RS) * C);
       }
       for (; r < r1; r += g.RS) {
         const long long o = base + r * C;
         const GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), d = gn_ld<T, VEC>(dout + o);
         GnVec<T, VEC> w;
         if (wr) w = gn_ld<T, VEC>(res + o);
-        row(v, d, w);
+        row(v, d, w, o);
       }
-      // sum g (x - mh) -> sum g xh
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) b[e] = (b[e] - k.ml[UG ? 0 : e] * a[e]) * k.r[UG ? 0 : e];
+      for (int e = 0; e < VEC; ++e) b[e] = gn_centre(b[e], a[e], stn[(vec * VEC + (UG ? 0 : e)) / D]);
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -341,7 +338,7 @@ __global__ void __launch_bounds__(256)
 gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout, T* __restrict__ dx,
                     T* __restrict__ dres, const float* __restrict__ gamma, const float* __restrict__ beta,
                     const GnStat* __restrict__ stats, const float2* __restrict__ ab, long long S, int C, int G, int chunks,
-                    double cap) {
+                    float cap) {
   constexpr int U = 2;
   const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
   const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
@@ -350,27 +347,26 @@ gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, const T*
   if (g.rl >= g.RS) return;
   for (int vec = g.col; vec < vpr; vec += g.VT) {
     GnCoef<VEC, UG> k;
-    typename GnBorderOf<ACT, VEC>::type bd;
-    k.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
-    bd.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
-    float pa[k.NG], pb[k.NG];  // dx = g*sc + pa + (x - mh)*pb
+    const GnStat* stn = stats + (long long)n * G;
+    k.load(stn, gamma, beta, vec * VEC, D);
+    float pa[k.NG], pb[k.NG];
 #pragma unroll
     for (int i = 0; i < k.NG; ++i) {
-      const float2 v = ab[(long long)n * G + (vec * VEC + i) / D];
-      pb[i] = -v.y * k.r[i] * k.r[i];
-      pa[i] = -v.x * k.r[i] - k.ml[i] * pb[i];
+      const int gi = (vec * VEC + i) / D;
+      const float2 v = ab[(long long)n * G + gi];
+      gn_dx_coefs(v.x, v.y, stn[gi], pa[i], pb[i]);
     }
     const long long base = (long long)n * S * C + (long long)vec * VEC;
     const bool wr = ACT != GN_NONE && res;
-    const auto row = [&](GnVec<T, VEC>& v, GnVec<T, VEC>& d, const GnVec<T, VEC>& w) {
+    const auto row = [&](GnVec<T, VEC>& v, GnVec<T, VEC>& d, const GnVec<T, VEC>& w, long long o) {
+      float gr[VEC];
+      gn_grads<ACT>(gr, d, v, w, wr, k, x + o, res + o, stn, gamma, beta, vec * VEC, D, cap);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const int i = UG ? 0 : e;
-        const float xf = ElemTraits<T>::to_f32(v.v[e]), t = xf - k.mh[i];
-        const float gr = gn_grad<ACT, VEC>(ElemTraits<T>::to_f32(d.v[e]), xf, t, wr ? ElemTraits<T>::to_f32(w.v[e]) : 0.f,
-                                           k.sc[e], k.sh[e], bd, e, cap);
-        v.v[e] = ElemTraits<T>::from_f32(gr * k.sc[e] + (t * pb[i] + pa[i]));
-        d.v[e] = ElemTraits<T>::from_f32(gr);
+        const float t = ElemTraits<T>::to_f32(v.v[e]) - k.mh[i];
+        v.v[e] = ElemTraits<T>::from_f32(gr[e] * k.sc[e] + (t * pb[i] + pa[i]));
+        d.v[e] = ElemTraits<T>::from_f32(gr[e]);
       }
     };
     long long r = r0 + g.rl;
@@ -386,7 +382,7 @@ gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, const T*
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long long o = base + (r + u * g.RS) * C;
-        row(v[u], d[u], w[u]);
+        row(v[u], d[u], w[u], o);
         gn_st<T, VEC>(dx + o, v[u]);
         if (dres) gn_st<T, VEC>(dres + o, d[u]);
       }
@@ -395,7 +391,7 @@ gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, const T*
       const long long o = base + r * C;
       GnVec<T, VEC> v = gn_ld<T, VEC>(x + o), d = gn_ld<T, VEC>(dout + o), w;
       if (wr) w = gn_ld<T, VEC>(res + o);
-      row(v, d, w);
+      row(v, d, w, o);
       gn_st<T, VEC>(dx + o, v);
       if (dres) gn_st<T, VEC>(dres + o, d);
     }
@@ -415,7 +411,7 @@ int gn_vec(int C, int esize, std::initializer_list<const void*> ptrs) {
 
 // act: 0 none, 1 ReLU, 2 ReLU clipped at cap, 3 SiLU (the codes of the Python side)
 bool gn_args_ok(long long N, long long S, int C, int G, int chunks, int act) {
-  return N > 0 && S > 0 && C > 0 && G > 0 && C % G == 0 && chunks > 0 && chunks <= S && act >= 0 && act <= 3 &&
+  return N > 0 && S > 0 && C > 0 && G > 0 && C % G == 0 && chunks >= 0 && chunks <= S && act >= 0 && act <= 3 &&
          N * chunks < (1ll << 31) && N * G < (1ll << 31);
 }
 int gn_act_class(int act, float& cap) {
@@ -449,47 +445,72 @@ int gn_act_class(int act, float& cap) {
   if (ug && VEC * sizeof(E) == 16) { constexpr bool UG = VEC * sizeof(E) == 16; __VA_ARGS__; }                \
   else { constexpr bool UG = false; __VA_ARGS__; }
 
-// Row chunks per sample: about 2048 blocks over the chip, at least 8 rows for each thread of a block.
-PDA_EXPORT int pda_group_norm_chunks(int dtype, long long N, long long S, int C) {
-  if (N <= 0 || S <= 0 || C <= 0) return -1;
-  const int vpr = (C * (dtype == PDA_F32 ? 4 : 2) + 15) / 16;
+// How a call runs: 0 = a slab of a sample in registers (group_norm_resident.h), > 0 = that many row chunks a sample, in
+// passes.  aligned: every tensor starts on 16 bytes.
+PDA_EXPORT int pda_group_norm_plan(int dtype, long long N, long long S, int C, int G, int bwd, int aligned) {
+  if (N <= 0 || S <= 0 || C <= 0 || G <= 0 || C % G) return -1;
+  const int es = dtype == PDA_F32 ? 4 : 2;
+  if (aligned && gn_resident_plan(es, N, S, C, G, bwd != 0).nv) return 0;
+  // about 2048 blocks over the chip, at least 8 rows for each thread of a block
+  const int vpr = (C * es + 15) / 16;
   const int rs = vpr >= 256 ? 1 : 256 / vpr;
   long long want = (2048 + N - 1) / N, most = S / (rs * 8ll);
   if (want > most) want = most;
   return (int)(want < 1 ? 1 : want > 1024 ? 1024 : want);
 }
 
-// part: two fp64 [N][chunks][C]; stats: {fp64 mean, fp64 1/std} [N][G]
+// chunks: from pda_group_norm_plan, as are those of the backward pass.  part: two fp64 [N][chunks][C] (none at 0 chunks);
+// stats: {fp64 mean, fp64 1/std} [N][G]
 PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x, const void* res, void* out, const float* gamma,
                                   const float* beta, long long N, long long S, int C, int G, double eps, int act, float cap,
                                   int chunks, void* part, void* stats, hipStream_t st) {
   if (!gn_args_ok(N, S, C, G, chunks, act)) return -1;
   const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, out});
+  const int cls = gn_act_class(act, cap);
+  if (chunks == 0) {
+    const GnPlan p = gn_resident_plan(dtype == PDA_F32 ? 4 : 2, N, S, C, G, false);
+    if (!p.nv || vec * (dtype == PDA_F32 ? 4 : 2) != 16 || N * (C / p.W) >= (1ll << 31)) return -1;
+    const GnResidentArgs a{x, res, nullptr, out, nullptr, nullptr, gamma, beta, N, S, C, G, cls, eps, cap, (GnStat*)stats,
+                           nullptr, st};
+    return dtype == PDA_F32 ? gn_resident_fwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_fwd<f16>(p, a)
+           : dtype == PDA_BF16 ? gn_resident_fwd<bf16>(p, a) : -6;
+  }
   const int blocks = (int)(N * chunks);
   GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x, S, C,
                                              chunks, (GnSums*)part));
   GN_DISPATCH(dtype, 1, hipLaunchKernelGGL((gn_finalize_kernel<E>), dim3((int)(N * G)), dim3(64), 0, st, (const E*)x,
                                            (const GnSums*)part, S, C, G, chunks, eps, (GnStat*)stats));
-  const int cls = gn_act_class(act, cap);
   const bool ug = (C / G) % vec == 0;
   GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_apply_kernel<E, VEC, UG, ACT>), dim3(blocks), dim3(256),
               0, st, (const E*)x, (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, cap)));
   return pda_check_launch();
 }
 
-// part: float2 [N][chunks][C]; ab: float2 [N][G].  dgamma / dbeta: both or none.
+// part: float2 [N][max(chunks, 1)][C]; ab: float2 [N][G] (none at 0 chunks).  dgamma / dbeta: both or none.
 PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x, const void* res, const void* dout, void* dx, void* dres,
                                   const float* gamma, const float* beta, const void* stats, long long N, long long S, int C,
                                   int G, int act, float cap, int chunks, void* part, void* ab, float* dgamma, float* dbeta,
                                   hipStream_t st) {
   if (!gn_args_ok(N, S, C, G, chunks, act) || (dres && !dx)) return -1;
   const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, dout, dx, dres});
-  const int blocks = (int)(N * chunks);
   const int cls = gn_act_class(act, cap);
+  if (chunks == 0) {
+    const GnPlan p = gn_resident_plan(dtype == PDA_F32 ? 4 : 2, N, S, C, G, true);
+    if (!p.nv || vec * (dtype == PDA_F32 ? 4 : 2) != 16 || N * (C / p.W) >= (1ll << 31)) return -1;
+    const GnResidentArgs a{x, res, dout, nullptr, dx, dres, gamma, beta, N, S, C, G, cls, 0.0, cap, (GnStat*)const_cast<void*>(stats),
+                           dgamma ? (float2*)part : nullptr, st};
+    const int rc = dtype == PDA_F32 ? gn_resident_bwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_bwd<f16>(p, a)
+                   : dtype == PDA_BF16 ? gn_resident_bwd<bf16>(p, a) : -6;
+    if (rc) return rc;
+    if (dgamma)
+      hipLaunchKernelGGL(gn_params_kernel, dim3((C + 3) / 4), dim3(1024), 0, st, (const float2*)part, N, C, dgamma, dbeta);
+    return pda_check_launch();
+  }
+  const int blocks = (int)(N * chunks);
   const bool ug = (C / G) % vec == 0;
   GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_bwd_partial_kernel<E, VEC, UG, ACT>), dim3(blocks),
               dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, gamma, beta, (const GnStat*)stats, S, C, G, chunks,
-              (double)cap, (float2*)part)));
+              cap, (float2*)part)));
   hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const float2*)part, gamma, S, C, G, chunks,
                      (float2*)ab);
   if (dgamma)
@@ -498,6 +519,6 @@ PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x, const void* res, con
   if (dx)
     GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_bwd_apply_kernel<E, VEC, UG, ACT>), dim3(blocks),
                 dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, (E*)dx, (E*)dres, gamma, beta,
-                (const GnStat*)stats, (const float2*)ab, S, C, G, chunks, (double)cap)));
+                (const GnStat*)stats, (const float2*)ab, S, C, G, chunks, cap)));
   return pda_check_launch();
 }

@@ -94,7 +94,7 @@ _SIGS = {
     "pda_gap_fwd": [c_i, c_p, c_p, c_i, c_i, c_i, c_p],
     "pda_gap_bwd": [c_i, c_p, c_p, c_i, c_i, c_i, c_p],
     "pda_softmax_ce": [c_i, c_p, c_p, c_i, c_i, c_f, c_p, c_p, c_p, c_p, c_p],
-    "pda_group_norm_chunks": [c_i, c_ll, c_ll, c_i],
+    "pda_group_norm_plan": [c_i, c_ll, c_ll, c_i, c_i, c_i, c_i],
     "pda_group_norm_fwd": [c_i, c_p, c_p, c_p, c_p, c_p, c_ll, c_ll, c_i, c_i, c_d, c_i, c_f, c_i, c_p, c_p, c_p],
     "pda_group_norm_bwd": [c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_f, c_i, c_p, c_p, c_p,
                            c_p, c_p],

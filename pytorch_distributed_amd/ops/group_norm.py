@@ -56,6 +56,15 @@ def _check(x, num_groups, gamma, beta, residual, eps) -> int:
     return groups
 
 
+def _plan(l, x, S: int, groups: int, backward: bool, *others) -> int:
+    """0: a sample's groups stay in registers; otherwise the row chunks of the multi-pass kernels."""
+    aligned = all(t is None or t.data_ptr() % 16 == 0 for t in (x,) + others)
+    chunks = l.pda_group_norm_plan(_lib.dt(x), x.shape[0], S, x.shape[-1], groups, int(backward), int(aligned))
+    if chunks < 0:
+        _lib.check(chunks, "pda_group_norm_plan")
+    return chunks
+
+
 def _f32(p):
     return None if p is None else p.detach().float().contiguous()
 
@@ -71,14 +80,13 @@ class _GroupNormActFn(torch.autograd.Function):
         out = torch.empty_like(x)
         ga, be = _f32(gamma), _f32(beta)
         with torch.cuda.device(x.device):
-            chunks = l.pda_group_norm_chunks(_lib.dt(x), N, S, C)
-            part = torch.empty((N * chunks, C, 2), device=x.device, dtype=torch.float64)
+            chunks = _plan(l, x, S, groups, False, residual)
+            part = torch.empty((N * chunks, C, 2), device=x.device, dtype=torch.float64) if chunks else None
             stats = torch.empty((N, groups, 2), device=x.device, dtype=torch.float64)
             _lib.check(l.pda_group_norm_fwd(_lib.dt(x), x.data_ptr(), _lib.ptr(residual), out.data_ptr(), _lib.ptr(ga),
-                                            _lib.ptr(be), N, S, C, groups, eps, act, cap, chunks, part.data_ptr(),
+                                            _lib.ptr(be), N, S, C, groups, eps, act, cap, chunks, _lib.ptr(part),
                                             stats.data_ptr(), _lib.stream()), "pda_group_norm_fwd")
-        ctx.cfg = (groups, act, cap, chunks)
-        ctx.has_res = residual is not None
+        ctx.cfg = (groups, act, cap)
         # with no activation the residual passes its gradient on unread
         ctx.save_for_backward(x, gamma, beta, residual if act else None, stats)
         return out
@@ -88,7 +96,7 @@ class _GroupNormActFn(torch.autograd.Function):
     def backward(ctx, dout):
         l = _lib.lib()
         x, gamma, beta, residual, stats = ctx.saved_tensors
-        groups, act, cap, chunks = ctx.cfg
+        groups, act, cap = ctx.cfg
         dout = dout.contiguous()
         N, C = x.shape[0], x.shape[-1]
         S = x.numel() // (N * C)
@@ -103,11 +111,12 @@ class _GroupNormActFn(torch.autograd.Function):
             if want_g or want_b:
                 dgb = torch.empty((2, C), device=x.device, dtype=torch.float32)
             if dx is not None or dgb is not None:
-                part = torch.empty((N * chunks, C, 2), device=x.device, dtype=torch.float32)
-                ab = torch.empty((N, groups, 2), device=x.device, dtype=torch.float32)
+                chunks = _plan(l, x, S, groups, True, residual, dout)
+                part = torch.empty((N * max(chunks, 1), C, 2), device=x.device, dtype=torch.float32)
+                ab = torch.empty((N, groups, 2), device=x.device, dtype=torch.float32) if chunks else None
                 _lib.check(l.pda_group_norm_bwd(_lib.dt(x), x.data_ptr(), _lib.ptr(residual), dout.data_ptr(), _lib.ptr(dx),
                                                 _lib.ptr(dres) if act else 0, _lib.ptr(ga), _lib.ptr(be), stats.data_ptr(),
-                                                N, S, C, groups, act, cap, chunks, part.data_ptr(), ab.data_ptr(),
+                                                N, S, C, groups, act, cap, chunks, part.data_ptr(), _lib.ptr(ab),
                                                 0 if dgb is None else dgb[0].data_ptr(),
                                                 0 if dgb is None else dgb[1].data_ptr(), _lib.stream()),
                            "pda_group_norm_bwd")
