@@ -6,8 +6,11 @@
 #pragma once
 #include "common.h"
 
-// Activation classes.  GN_CAP is every clipped ReLU; the plain one is clipped at infinity.
-enum GnAct : int { GN_NONE = 0, GN_CAP = 1, GN_SILU = 2 };
+#include <math.h>
+
+// Activations (the codes of the Python side).
+enum GnAct : int { GN_NONE = 0, GN_RELU = 1, GN_CAP = 2, GN_SILU = 3 };
+constexpr bool gn_is_relu(int act) { return act == GN_RELU || act == GN_CAP; }
 
 struct GnStat { double mean, rstd; };
 
@@ -25,6 +28,24 @@ template <typename T> struct GnRaw {
     else {
       const unsigned short h = (unsigned short)(e & 1 ? u[e >> 1] >> 16 : u[e >> 1]);
       return ElemTraits<T>::to_f32(__builtin_bit_cast(T, h));
+    }
+  }
+  // f(e) - s.  fp16: one multiply-add that reads the half where it lies (one: 1.0 that the compiler does not see as such)
+  __device__ __forceinline__ float sub(int e, float s, float one) const {
+    if constexpr (sizeof(T) == 2 && ElemTraits<T>::code == PDA_F16) return __builtin_fmaf(f(e), one, -s);
+    return f(e) - s;
+  }
+  // a + f(e)
+  __device__ __forceinline__ float add(int e, float a, float one) const {
+    if constexpr (sizeof(T) == 2 && ElemTraits<T>::code == PDA_F16) return __builtin_fmaf(f(e), one, a);
+    return f(e) + a;
+  }
+  // elements whose bit is not set become 0
+  __device__ __forceinline__ void keep(const bool (&on)[16 / sizeof(T)]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) u[i] = on[i] ? u[i] : 0u;
+      else u[i] &= (on[2 * i] ? 0xffffu : 0u) | (on[2 * i + 1] ? 0xffff0000u : 0u);
     }
   }
   __device__ __forceinline__ void set(const float (&x)[16 / sizeof(T)]) {
@@ -49,6 +70,12 @@ __device__ __forceinline__ void gn_st(T* p, const GnVec<T, VEC>& v) { *reinterpr
 template <int VEC, bool UG> struct GnCoef {
   static constexpr int NG = UG ? 1 : VEC;
   float mh[NG], sc[VEC], sh[VEC];
+  __device__ __forceinline__ float shmax() const {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) m = fmaxf(m, fabsf(sh[e]));
+    return m;
+  }
   __device__ __forceinline__ void load(const GnStat* st /* of this sample */, const float* gamma, const float* beta, int c0,
                                        int D) {
 #pragma unroll
@@ -79,10 +106,8 @@ __device__ __forceinline__ float gn_sigmoid(float z) {
 
 template <int ACT> __device__ __forceinline__ float gn_act(float z, float cap) {
   if constexpr (ACT == GN_SILU) return z * gn_sigmoid(z);
-  if constexpr (ACT == GN_CAP) {
-    z = z < 0.f ? 0.f : z;      // a NaN stays one
-    z = z > cap ? cap : z;
-  }
+  if constexpr (gn_is_relu(ACT)) z = z < 0.f ? 0.f : z;  // a NaN stays one
+  if constexpr (ACT == GN_CAP) z = z > cap ? cap : z;
   return z;
 }
 
@@ -101,27 +126,29 @@ __device__ __forceinline__ unsigned gn_inside(const T* x, const T* res, const Gn
   return on;
 }
 
-// act'(z) of the clipped ReLU for a vector: one bit an element, and whether one lies so near a border of the activation (16
-// fp32 roundings of its parts) that gn_inside has to decide: on which side it lies decides over its whole gradient.
-template <typename V, int VEC, bool UG>
-__device__ __forceinline__ unsigned gn_bits(const V& v, const V& w, bool wr, const GnCoef<VEC, UG>& k, float cap, bool& near) {
-  unsigned on = 0;
-  near = false;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const float t = (v.f(e) - k.mh[UG ? 0 : e]) * k.sc[e];
-    float z = t + k.sh[e];
-    if (wr) z += w.f(e);
-    // (at 0 a residual is as large as t + sh; at the cap it is at most that and the cap)
-    const float a = fabsf(t) + fabsf(k.sh[e]);
-    near |= fabsf(z) < 1e-6f * a || fabsf(z - cap) < 1e-6f * (a + cap);
-    on |= z > 0.f && z < cap ? 1u << e : 0u;
+// The ReLUs' act'(z) of one element, and what decides whether its vector is looked at again: on which side of a border z
+// lies decides over an element's whole gradient.  With z = t + sh + res, z's rounding error is below 6 u (|t| + |sh| + |res|),
+// u = 2^-24, and next to 0 |t| is at most |sh| + |res| (next to the cap: and the cap).  So a vector whose least |z| is below
+// 2e-6 (max |sh| + max |res|) is decided by gn_inside.
+struct GnNear {
+  float lo = INFINITY, hi = INFINITY, res = 0.f;
+  template <int ACT> __device__ __forceinline__ bool inside(float z, float cap) {
+    lo = fminf(lo, fabsf(z));
+    if constexpr (ACT == GN_CAP) {
+      hi = fminf(hi, fabsf(z - cap));
+      return z > 0.f && z < cap;
+    }
+    return z > 0.f;
   }
-  return on;
-}
+  template <int ACT> __device__ __forceinline__ bool again(float shmax, float cap) const {
+    const float tol = 2e-6f * (shmax + res);
+    return lo < tol || (ACT == GN_CAP && hi < tol + 2e-6f * cap);
+  }
+};
+// t = x - mh
 template <typename V, int VEC, bool UG>
-__device__ __forceinline__ float gn_silu_slope(const V& v, const V& w, bool wr, const GnCoef<VEC, UG>& k, int e) {
-  float z = (v.f(e) - k.mh[UG ? 0 : e]) * k.sc[e] + k.sh[e];
+__device__ __forceinline__ float gn_silu_slope(float t, const V& w, bool wr, const GnCoef<VEC, UG>& k, int e) {
+  float z = t * k.sc[e] + k.sh[e];
   if (wr) z += w.f(e);
   const float s = gn_sigmoid(z);
   return s * (1.f + z * (1.f - s));
@@ -133,17 +160,26 @@ __device__ __forceinline__ void gn_grads(float (&g)[VEC], const GnVec<T, VEC>& d
                                          bool wr, const GnCoef<VEC, UG>& k, const T* x, const T* res, const GnStat* st,
                                          const float* gamma, const float* beta, int c0, int D, float cap) {
   unsigned on = 0;
-  if constexpr (ACT == GN_CAP) {
-    bool near;
-    on = gn_bits(v, w, wr, k, cap, near);
-    if (near) on = gn_inside<T, VEC>(x, wr ? res : nullptr, st, gamma, beta, c0, D, cap);
+  if constexpr (gn_is_relu(ACT)) {
+    GnNear near;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float z = (v.f(e) - k.mh[UG ? 0 : e]) * k.sc[e] + k.sh[e];
+      if (wr) {
+        const float r = w.f(e);
+        z += r;
+        near.res = fmaxf(near.res, fabsf(r));
+      }
+      on |= near.inside<ACT>(z, cap) ? 1u << e : 0u;
+    }
+    if (near.again<ACT>(k.shmax(), cap)) on = gn_inside<T, VEC>(x, wr ? res : nullptr, st, gamma, beta, c0, D, cap);
   }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
     const float dy = ElemTraits<T>::to_f32(d.v[e]);
     if constexpr (ACT == GN_NONE) g[e] = dy;
-    if constexpr (ACT == GN_CAP) g[e] = (on >> e) & 1u ? dy : 0.f;
-    if constexpr (ACT == GN_SILU) g[e] = dy * gn_silu_slope(v, w, wr, k, e);
+    if constexpr (gn_is_relu(ACT)) g[e] = (on >> e) & 1u ? dy : 0.f;
+    if constexpr (ACT == GN_SILU) g[e] = dy * gn_silu_slope(v.f(e) - k.mh[UG ? 0 : e], w, wr, k, e);
   }
 }
 

@@ -409,14 +409,9 @@ int gn_vec(int C, int esize, std::initializer_list<const void*> ptrs) {
   return 1;
 }
 
-// act: 0 none, 1 ReLU, 2 ReLU clipped at cap, 3 SiLU (the codes of the Python side)
 bool gn_args_ok(long long N, long long S, int C, int G, int chunks, int act) {
-  return N > 0 && S > 0 && C > 0 && G > 0 && C % G == 0 && chunks >= 0 && chunks <= S && act >= 0 && act <= 3 &&
+  return N > 0 && S > 0 && C > 0 && G > 0 && C % G == 0 && chunks >= 0 && chunks <= S && act >= GN_NONE && act <= GN_SILU &&
          N * chunks < (1ll << 31) && N * G < (1ll << 31);
-}
-int gn_act_class(int act, float& cap) {
-  if (act == 1) cap = INFINITY;
-  return act == 0 ? GN_NONE : act == 3 ? GN_SILU : GN_CAP;
 }
 
 }  // namespace
@@ -438,6 +433,7 @@ int gn_act_class(int act, float& cap) {
 #define GN_DISPATCH_ACT(act, ug, ...)                                                          \
   switch (act) {                                                                               \
     case GN_NONE: { constexpr int ACT = GN_NONE; GN_UG(ug, __VA_ARGS__) } break;               \
+    case GN_RELU: { constexpr int ACT = GN_RELU; GN_UG(ug, __VA_ARGS__) } break;               \
     case GN_CAP: { constexpr int ACT = GN_CAP; GN_UG(ug, __VA_ARGS__) } break;                 \
     default: { constexpr int ACT = GN_SILU; GN_UG(ug, __VA_ARGS__) } break;                    \
   }
@@ -466,11 +462,10 @@ PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x, const void* res, voi
                                   int chunks, void* part, void* stats, hipStream_t st) {
   if (!gn_args_ok(N, S, C, G, chunks, act)) return -1;
   const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, out});
-  const int cls = gn_act_class(act, cap);
   if (chunks == 0) {
     const GnPlan p = gn_resident_plan(dtype == PDA_F32 ? 4 : 2, N, S, C, G, false);
     if (!p.nv || vec * (dtype == PDA_F32 ? 4 : 2) != 16 || N * (C / p.W) >= (1ll << 31)) return -1;
-    const GnResidentArgs a{x, res, nullptr, out, nullptr, nullptr, gamma, beta, N, S, C, G, cls, eps, cap, (GnStat*)stats,
+    const GnResidentArgs a{x, res, nullptr, out, nullptr, nullptr, gamma, beta, N, S, C, G, act, eps, cap, (GnStat*)stats,
                            nullptr, st};
     return dtype == PDA_F32 ? gn_resident_fwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_fwd<f16>(p, a)
            : dtype == PDA_BF16 ? gn_resident_fwd<bf16>(p, a) : -6;
@@ -481,7 +476,7 @@ PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x, const void* res, voi
   GN_DISPATCH(dtype, 1, hipLaunchKernelGGL((gn_finalize_kernel<E>), dim3((int)(N * G)), dim3(64), 0, st, (const E*)x,
                                            (const GnSums*)part, S, C, G, chunks, eps, (GnStat*)stats));
   const bool ug = (C / G) % vec == 0;
-  GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_apply_kernel<E, VEC, UG, ACT>), dim3(blocks), dim3(256),
+  GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_apply_kernel<E, VEC, UG, ACT>), dim3(blocks), dim3(256),
               0, st, (const E*)x, (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, cap)));
   return pda_check_launch();
 }
@@ -493,11 +488,10 @@ PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x, const void* res, con
                                   hipStream_t st) {
   if (!gn_args_ok(N, S, C, G, chunks, act) || (dres && !dx)) return -1;
   const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, dout, dx, dres});
-  const int cls = gn_act_class(act, cap);
   if (chunks == 0) {
     const GnPlan p = gn_resident_plan(dtype == PDA_F32 ? 4 : 2, N, S, C, G, true);
     if (!p.nv || vec * (dtype == PDA_F32 ? 4 : 2) != 16 || N * (C / p.W) >= (1ll << 31)) return -1;
-    const GnResidentArgs a{x, res, dout, nullptr, dx, dres, gamma, beta, N, S, C, G, cls, 0.0, cap, (GnStat*)const_cast<void*>(stats),
+    const GnResidentArgs a{x, res, dout, nullptr, dx, dres, gamma, beta, N, S, C, G, act, 0.0, act == GN_CAP ? cap : INFINITY, (GnStat*)const_cast<void*>(stats),
                            dgamma ? (float2*)part : nullptr, st};
     const int rc = dtype == PDA_F32 ? gn_resident_bwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_bwd<f16>(p, a)
                    : dtype == PDA_BF16 ? gn_resident_bwd<bf16>(p, a) : -6;
@@ -508,17 +502,18 @@ PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x, const void* res, con
   }
   const int blocks = (int)(N * chunks);
   const bool ug = (C / G) % vec == 0;
-  GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_bwd_partial_kernel<E, VEC, UG, ACT>), dim3(blocks),
+  GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_bwd_partial_kernel<E, VEC, UG, ACT>), dim3(blocks),
               dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, gamma, beta, (const GnStat*)stats, S, C, G, chunks,
-              cap, (float2*)part)));
+              act == GN_CAP ? cap : INFINITY, (float2*)part)));
   hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const float2*)part, gamma, S, C, G, chunks,
                      (float2*)ab);
   if (dgamma)
     hipLaunchKernelGGL(gn_params_kernel, dim3((C + 3) / 4), dim3(1024), 0, st, (const float2*)part, N * chunks, C, dgamma,
                        dbeta);
   if (dx)
-    GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(cls, ug, hipLaunchKernelGGL((gn_bwd_apply_kernel<E, VEC, UG, ACT>), dim3(blocks),
+    GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_bwd_apply_kernel<E, VEC, UG, ACT>), dim3(blocks),
                 dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, (E*)dx, (E*)dres, gamma, beta,
-                (const GnStat*)stats, (const float2*)ab, S, C, G, chunks, cap)));
+                (const GnStat*)stats, (const float2*)ab, S, C, G, chunks,
+                act == GN_CAP ? cap : INFINITY)));
   return pda_check_launch();
 }

@@ -14,9 +14,14 @@ struct GnPlan {
   int W, threads, nv;  // nv = 0: does not fit
 };
 
-// Resident vectors of one thread: what stays below the 128 registers that 1024 threads leave each.
-constexpr int GN_NV_FWD = 13, GN_NV_BWD = 7;
+// Resident vectors of one thread: what stays below the 128 registers that 1024 threads leave each.  Backward, up to
+// GN_NV_BOTH vectors of x and dout stay; above that x alone does, and dout is read again (it has just passed through the
+// caches).
+constexpr int GN_NV_FWD = 13, GN_NV_BWD = 13, GN_NV_BOTH = 7;
 
+// Measured on 400 samples, fp16, forward / backward: the width of a slab's rows counts most (56x56x256 with residual:
+// 16 bytes 701 / 1381 us, 32 bytes 530 / 973, 64 bytes 443 us forward), up to 128 bytes (14x14x1024: 32 bytes 114 / 202, 64 bytes
+// 101 / 183, 128 bytes 108 / 194), then few threads with many vectors (28x28x512: 512 threads 197, 1024 230 us).
 inline GnPlan gn_resident_plan(int esize, long long N, long long S, int C, int G, bool bwd) {
   GnPlan best{0, 0, 0};
   const int vec = 16 / esize, D = C / G;
@@ -24,33 +29,47 @@ inline GnPlan gn_resident_plan(int esize, long long N, long long S, int C, int G
   int a = D, b = vec;
   while (b) { const int t = a % b; a = b; b = t; }
   const int unit = D / a * vec;  // whole groups and whole vectors
-  const int units = C / unit, most = bwd ? GN_NV_BWD : GN_NV_FWD;
-  for (int k = units; k >= 1; --k) {
+  const int units = C / unit;
+  double top = 0.0;
+  for (int k = 1; k <= units; ++k) {
     if (units % k) continue;
-    const int W = unit * k, vt = W / vec;
-    if (vt > 1024 || (W * esize < 32 && W != C)) continue;
-    int threads = 0;
-    for (int nt = 64; nt <= 1024 && !threads; nt *= 2)
-      if (nt >= vt && (S + nt / vt - 1) / (nt / vt) <= most) threads = nt;
+    const int W = unit * k, vt = W / vec, row = W * esize;
+    if (vt > 1024 || (row < 32 && W != C)) continue;
+    const long long blocks = N * (units / k);
+    // both tensors in registers where 512 threads do (two workgroups on a CU), else x alone
+    int threads = 0, most = bwd ? GN_NV_BOTH : GN_NV_FWD;
+    for (int pass = 0; pass < 2 && !threads; ++pass) {
+      for (int nt = 64; nt <= (bwd && pass == 0 ? 512 : 1024) && !threads; nt *= 2)
+        if (nt >= vt && (S + nt / vt - 1) / (nt / vt) <= most) threads = nt;
+      most = bwd ? GN_NV_BWD : GN_NV_FWD;
+    }
     if (!threads) continue;
-    // spread a slab over more threads while the vectors of each stay two or more
-    while (threads < 1024 && (S + threads / vt - 1) / (threads / vt) > 4 && S * vt <= 2048) threads *= 2;
+    // few blocks: more threads each, while their vectors stay two or more
+    while (threads < 1024 && blocks * threads < 256 * 512 && (S + threads / vt - 1) / (threads / vt) > 3) threads *= 2;
     const int nv = (int)((S + threads / vt - 1) / (threads / vt));
-    best = GnPlan{W, threads, nv};
-    // wide enough a launch, and two workgroups or more on a CU, so that one's loads cover the other's sums
-    if (N * (units / k) >= 1024 && threads <= 512) break;
+    const double fill = (double)blocks * threads / (256.0 * 512.0), used = (double)(S * vt) / ((double)threads * nv);
+    double score = (row < 64 ? 0.75 : row < 128 ? 0.92 : row <= 256 ? 1.0 : 0.97) * (fill < 1.0 ? fill : 1.0);
+    score *= used;                                                          // rows that do not fill the block
+    if (S * vt < 256 && blocks > 1024) score *= sqrt((double)(S * vt) / 256.0);  // a workgroup costs, too
+    if (threads > 512) score *= D % vec ? 0.75 : 0.92;  // (several groups a vector: more registers, spills at 13 vectors)
+    if (bwd && nv > GN_NV_BOTH) score *= 0.9;
+    if (score > top) {
+      top = score;
+      best = GnPlan{W, threads, nv};
+    }
   }
   return best;
 }
 
 // Totals of every channel of the slab: buf [RS][W] (written, not yet synchronised) -> buf[0..W).  tmp: max(threads, W).
 template <typename V> __device__ __forceinline__ void gn_channel_totals(V* buf, V* tmp, int W, int RS) {
-  const int NT = blockDim.x, parts = NT > W ? NT / W : 1;
+  // (V: a number or a pair of them)
+  const int NT = blockDim.x, parts = NT < W ? 1 : NT / W < RS ? NT / W : RS;
   __syncthreads();
   for (int i = threadIdx.x; i < W * parts; i += NT) {
     const int c = i % W, p = i / W;
-    V a = 0;
-    for (int r = p; r < RS; r += parts) a += buf[r * W + c];
+    V a = buf[p * W + c];  // p < RS: a part has a row at least
+    for (int r = p + parts; r < RS; r += parts) a += buf[r * W + c];
     tmp[i] = a;
   }
   __syncthreads();
@@ -67,7 +86,7 @@ inline size_t gn_fwd_lds(int W, int threads, int vec, int D) {
   return 8ull * ((size_t)(threads / (W / vec)) * W + (threads > W ? threads : W) + 2 * (W / D));
 }
 inline size_t gn_bwd_lds(int W, int threads, int vec, int D) {
-  return 4ull * (2 * (size_t)(threads / (W / vec)) * W + 2 * (threads > W ? threads : W) + 2 * (W / D));
+  return 8ull * ((size_t)(threads / (W / vec)) * W + (threads > W ? threads : W) + W / D);
 }
 
 struct GnPair { double a, b; };
@@ -117,6 +136,36 @@ __device__ __forceinline__ void gn_group_totals(GnPair (&s)[UG ? 1 : VEC], doubl
     }
     __syncthreads();
     if (on) s[0] = grp[col / dv];
+  } else if (shuffles) {  // a vector holds whole groups (D divides it), columns are a power of two
+    GnPair* buf = reinterpret_cast<GnPair*>(lds);
+    const int per = VEC / D, c0 = col * per;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (!on) s[e] = GnPair{0.0, 0.0};
+    if (D > 1)  // into a group's first slot
+#pragma unroll
+      for (int e = 0; e + 1 < VEC; e += 2) s[e] = GnPair{s[e].a + s[e + 1].a, s[e].b + s[e + 1].b};
+    if (D > 2)
+#pragma unroll
+      for (int e = 0; e + 2 < VEC; e += 4) s[e] = GnPair{s[e].a + s[e + 2].a, s[e].b + s[e + 2].b};
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (e % D == 0) {
+        for (int o = VT; o < 64; o <<= 1) {
+          s[e].a += __shfl_xor(s[e].a, o, 64);
+          s[e].b += __shfl_xor(s[e].b, o, 64);
+        }
+        if (lane < VT) buf[wave * Gs + c0 + e / D] = s[e];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      s[e] = buf[c0 + e / D];
+      for (int w = 1; w < NW; ++w) {
+        s[e].a += buf[w * Gs + c0 + e / D].a;
+        s[e].b += buf[w * Gs + c0 + e / D].b;
+      }
+    }
   } else {
     double* tmp = lds + RS * W;
     double* grp = tmp + (blockDim.x > W ? blockDim.x : W);
@@ -154,6 +203,8 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
   const long long slab = (long long)n * S * C + c0;
   unsigned off = (unsigned)(rl * C + col * VEC);
   const auto at = [&](int i) { return slab + (long long)i * RS * C; };
+  float one = 1.f;
+  asm volatile("" : "+s"(one));
   GnRaw<T> v[NV];
   const auto in = [&](int i) { return on && rl + i * RS < S; };
 #pragma unroll
@@ -164,6 +215,9 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
   float s1[VEC], s2[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) s1[e] = s2[e] = 0.f;
+  float p0[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) p0[e] = v[0].f(e);
   int cnt = in(0) ? 1 : 0;
 #pragma unroll
   for (int i = 1; i < NV; ++i)
@@ -171,7 +225,7 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
       ++cnt;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = v[i].f(e) - v[0].f(e);
+        const float d = v[i].sub(e, p0[e], one);
         s1[e] += d;
         s2[e] += d * d;
       }
@@ -182,7 +236,7 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
   if (cnt)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const double p = (double)v[0].f(e), kp = (double)cnt * p, d = (double)s1[e];
+      const double p = (double)p0[e], kp = (double)cnt * p, d = (double)s1[e];
       tot[UG ? 0 : e].a += d + kp;
       tot[UG ? 0 : e].b += (double)s2[e] + p * (d + d + kp);
     }
@@ -222,8 +276,8 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
       float y[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float z = (v[i].f(e) - mh[UG ? 0 : e]) * sc[e] + sh[e];
-        if (res) z += w.f(e);
+        float z = v[i].sub(e, mh[UG ? 0 : e], one) * sc[e] + sh[e];
+        if (res) z = w.add(e, z, one);
         y[e] = gn_act<ACT>(z, cap);
       }
       v[i].set(y);
@@ -237,8 +291,9 @@ __global__ void __launch_bounds__(1024)
 gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout, T* __restrict__ dx,
                        T* __restrict__ dres, const float* __restrict__ gamma, const float* __restrict__ beta,
                        const GnStat* __restrict__ stats, int S, int C, int G, int W, float cap, float2* __restrict__ part) {
-  extern __shared__ float ldsf[];
+  extern __shared__ float2 lds2[];
   constexpr int VEC = 16 / sizeof(T);
+  constexpr bool BOTH = NV <= GN_NV_BOTH;  // x and dout stay; otherwise x and (ReLUs) one bit an element of act'(z)
   const int slabs = C / W, D = C / G, VT = W / VEC, RS = blockDim.x / VT, Gs = W / D;
   const int id = xcd_remap(blockIdx.x, gridDim.x), n = id / slabs, c0 = (id % slabs) * W;
   const int col = threadIdx.x % VT, rl = threadIdx.x / VT, ct = c0 + col * VEC;
@@ -249,97 +304,133 @@ gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const
   const auto in = [&](int i) { return on && rl + i * RS < S; };
   const bool wr = ACT != GN_NONE && res;
   const GnStat* stn = stats + (long long)n * G;
-  GnRaw<T> v[NV], d[NV];
+  float one = 1.f;
+  asm volatile("" : "+s"(one));
+  GnRaw<T> v[NV], d[BOTH ? NV : 1];
+  unsigned bits[BOTH ? 1 : (NV * VEC + 31) / 32];
+#pragma unroll
+  for (unsigned& q : bits) q = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (in(i)) {
       v[i] = gn_ld_raw<T>(x + at(i) + off);
-      d[i] = gn_ld_raw<T>(dout + at(i) + off);
+      if constexpr (BOTH) d[i] = gn_ld_raw<T>(dout + at(i) + off);
     }
   GnCoef<VEC, UG> k;
   k.load(stn, gamma, beta, on ? ct : c0, D);
   float a[VEC], b[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) a[e] = b[e] = 0.f;
-  // clipped ReLU: one bit an element says where g = dout, the rest is 0; vectors to be decided again are remembered
-  unsigned bits[(NV + 32 / VEC - 1) / (32 / VEC)], again = 0;
-#pragma unroll
-  for (unsigned& q : bits) q = 0;
+  // ReLUs: dout becomes g here (0 or as it was); vectors to be decided again are remembered
+  const float shmax = gn_is_relu(ACT) ? k.shmax() : 0.f;
+  unsigned again = 0;
   gn_renew(off);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (in(i)) {
       GnRaw<T> w;
+      GnRaw<T>& dy = d[BOTH ? i : 0];
       if (wr) w = gn_ld_raw<T>(res + at(i) + off);
-      unsigned on = 0;
-      if constexpr (ACT == GN_CAP) {
-        bool near;
-        on = gn_bits(v[i], w, wr, k, cap, near);
-        bits[i / (32 / VEC)] |= on << (i % (32 / VEC) * VEC);
-        again |= near ? 1u << i : 0u;
+      if constexpr (!BOTH) dy = gn_ld_raw<T>(dout + at(i) + off);
+      float t[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) t[e] = v[i].sub(e, k.mh[UG ? 0 : e], one);
+      if constexpr (gn_is_relu(ACT)) {
+        GnNear near;
+        bool on[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          float z = t[e] * k.sc[e] + k.sh[e];
+          if (wr) {
+            z = w.add(e, z, one);
+            near.res = fmaxf(near.res, fabsf(w.f(e)));
+          }
+          on[e] = near.inside<ACT>(z, cap);
+        }
+        dy.keep(on);
+        if constexpr (!BOTH)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) bits[(i * VEC + e) / 32] |= on[e] ? 1u << ((i * VEC + e) % 32) : 0u;
+        again |= near.again<ACT>(shmax, cap) ? 1u << i : 0u;
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float gr = d[i].f(e);
-        if constexpr (ACT == GN_CAP) gr = (on >> e) & 1u ? gr : 0.f;
-        if constexpr (ACT == GN_SILU) gr *= gn_silu_slope(v[i], w, wr, k, e);
-        a[e] += gr;
-        b[e] += gr * (v[i].f(e) - k.mh[UG ? 0 : e]);
+        if constexpr (ACT == GN_SILU) {
+          const float gr = dy.f(e) * gn_silu_slope(t[e], w, wr, k, e);
+          a[e] += gr;
+          b[e] += gr * t[e];
+        } else {
+          a[e] = dy.add(e, a[e], one);
+          b[e] = __builtin_fmaf(dy.f(e), t[e], b[e]);
+        }
       }
     }
-  float* bufa = ldsf;
-  float* bufb = bufa + RS * W;
-  float* tmp = bufb + RS * W;
-  const int nt = blockDim.x > W ? blockDim.x : W;
-  float* grp = tmp + 2 * nt;
+  float2* buf = lds2;
+  float2* tmp = buf + RS * W;
+  float2* grp = tmp + (blockDim.x > W ? blockDim.x : W);
   if (on)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      bufa[rl * W + col * VEC + e] = a[e];
-      bufb[rl * W + col * VEC + e] = gn_centre(b[e], a[e], stn[(UG ? ct : ct + e) / D]);
-    }
-  if constexpr (ACT == GN_CAP)
-    if (again) {  // rare: what fp64 says otherwise is taken from this thread's sums, and its bits are changed
+    for (int e = 0; e < VEC; ++e)
+      buf[rl * W + col * VEC + e] = make_float2(a[e], gn_centre(b[e], a[e], stn[(UG ? ct : ct + e) / D]));
+  if constexpr (gn_is_relu(ACT))
+    if (again) {  // rare: what fp64 says otherwise is put right in this thread's sums, in g and in the bits
 #pragma unroll 1
       for (int i = 0; i < NV; ++i) {
         if (!((again >> i) & 1u)) continue;
         const long long o = at(i) + off;
         const unsigned on = gn_inside<T, VEC>(x + o, wr ? res + o : nullptr, stn, gamma, beta, ct, D, cap);
-        unsigned old = 0;
+        unsigned was = 0;
 #pragma unroll
-        for (int q = 0; q < (int)(sizeof(bits) / 4); ++q)
-          if (i / (32 / VEC) == q) {
-            old = (bits[q] >> (i % (32 / VEC) * VEC)) & ((1u << VEC) - 1u);
-            bits[q] ^= (old ^ on) << (i % (32 / VEC) * VEC);
-          }
+        for (int j = 0; j < NV; ++j)
+          if (j == i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              if constexpr (BOTH) {
+                was |= d[j].f(e) != 0.f ? 1u << e : 0u;
+              } else {
+                const unsigned bit = 1u << ((j * VEC + e) % 32);
+                unsigned& q = bits[(j * VEC + e) / 32];
+                was |= q & bit ? 1u << e : 0u;
+                q = (on >> e) & 1u ? q | bit : q & ~bit;
+              }
+            }
 #pragma unroll 1
         for (int e = 0; e < VEC; ++e) {
-          if (!(((old ^ on) >> e) & 1u)) continue;
-          const float dy = ((on >> e) & 1u ? 1.f : -1.f) * ElemTraits<T>::to_f32(dout[o + e]);
+          const float dy = ElemTraits<T>::to_f32(dout[o + e]);
+          if (!(((on ^ was) >> e) & 1u) || dy == 0.f) continue;
+          const float more = (on >> e) & 1u ? dy : -dy;
           const GnStat st = stn[(ct + e) / D];
-          bufa[rl * W + col * VEC + e] += dy;
-          bufb[rl * W + col * VEC + e] += dy * (float)(((double)ElemTraits<T>::to_f32(x[o + e]) - st.mean) * st.rstd);
+          buf[rl * W + col * VEC + e] += make_float2(more, more * (float)(((double)ElemTraits<T>::to_f32(x[o + e]) - st.mean) * st.rstd));
+        }
+        if constexpr (BOTH) {
+          GnRaw<T> now = gn_ld_raw<T>(dout + o);
+          bool keep[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) keep[e] = (on >> e) & 1u;
+          now.keep(keep);
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            if (j == i) d[j] = now;
         }
       }
     }
-  gn_channel_totals(bufa, tmp, W, RS);
-  gn_channel_totals(bufb, tmp + nt, W, RS);
+  gn_channel_totals(buf, tmp, W, RS);
   if (part)
-    for (int c = threadIdx.x; c < W; c += blockDim.x) part[(long long)n * C + c0 + c] = make_float2(bufa[c], bufb[c]);
+    for (int c = threadIdx.x; c < W; c += blockDim.x) part[(long long)n * C + c0 + c] = buf[c];
   if (!dx) return;
   for (int g = threadIdx.x >> 6; g < Gs; g += blockDim.x >> 6) {
     double ta = 0.0, tb = 0.0;
     for (int j = threadIdx.x & 63; j < D; j += 64) {
       const double ga = gamma ? (double)gamma[c0 + g * D + j] : 1.0;
-      ta += ga * (double)bufa[g * D + j];
-      tb += ga * (double)bufb[g * D + j];
+      const float2 t = buf[g * D + j];
+      ta += ga * (double)t.x;
+      tb += ga * (double)t.y;
     }
     ta = wave_sum_f64(ta);
     tb = wave_sum_f64(tb);
     if ((threadIdx.x & 63) == 0) {
       const double m = (double)S * D;
-      grp[2 * g] = (float)(ta / m);
-      grp[2 * g + 1] = (float)(tb / m);
+      grp[g] = make_float2((float)(ta / m), (float)(tb / m));
     }
   }
   __syncthreads();
@@ -348,32 +439,40 @@ gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const
 #pragma unroll
   for (int i = 0; i < k.NG; ++i) {
     const int g = (col * VEC + i) / D;
-    gn_dx_coefs(grp[2 * g], grp[2 * g + 1], stn[c0 / D + g], pa[i], pb[i]);
+    gn_dx_coefs(grp[g].x, grp[g].y, stn[c0 / D + g], pa[i], pb[i]);
   }
   gn_renew(off);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     gn_renew(v[i]);
-    gn_renew(d[i]);
+    if constexpr (BOTH) gn_renew(d[i]);
     if (in(i)) {
       GnRaw<T> w;
+      GnRaw<T>& dy = d[BOTH ? i : 0];
+      if constexpr (!BOTH) {
+        dy = gn_ld_raw<T>(dout + at(i) + off);
+        if constexpr (gn_is_relu(ACT)) {
+          bool on[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) on[e] = (bits[(i * VEC + e) / 32] >> ((i * VEC + e) % 32)) & 1u;
+          dy.keep(on);
+        }
+      }
       if (ACT == GN_SILU && wr) w = gn_ld_raw<T>(res + at(i) + off);
       float y[VEC], gs[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const int j = UG ? 0 : e;
-        float gr = d[i].f(e);
-        if constexpr (ACT == GN_CAP) gr = (bits[i / (32 / VEC)] >> (i % (32 / VEC) * VEC + e)) & 1u ? gr : 0.f;
-        if constexpr (ACT == GN_SILU) gr *= gn_silu_slope(v[i], w, wr, k, e);
-        const float t = v[i].f(e) - k.mh[j];
-        y[e] = gr * k.sc[e] + (t * pb[j] + pa[j]);
-        gs[e] = gr;
+        const float t = v[i].sub(e, k.mh[j], one);
+        gs[e] = ACT == GN_SILU ? dy.f(e) * gn_silu_slope(t, w, wr, k, e) : 0.f;
+        const float rest = t * pb[j] + pa[j];
+        y[e] = ACT == GN_SILU ? gs[e] * k.sc[e] + rest : __builtin_fmaf(dy.f(e), k.sc[e], rest);
       }
       v[i].set(y);
       gn_st_raw<T>(dx + at(i) + off, v[i]);
       if (dres) {
-        d[i].set(gs);
-        gn_st_raw<T>(dres + at(i) + off, d[i]);
+        if constexpr (ACT == GN_SILU) dy.set(gs);
+        gn_st_raw<T>(dres + at(i) + off, dy);
       }
     }
   }
@@ -404,7 +503,7 @@ template <typename K> static int gn_allow_lds(K kernel, size_t lds) {
 template <typename T, int NV, bool UG, int ACT> static int gn_launch_fwd(const GnPlan& p, const GnResidentArgs& a) {
   constexpr int VEC = 16 / sizeof(T);
   const int D = a.C / a.G, vt = p.W / VEC, dv = D / VEC;
-  const int shuffles = UG && vt <= 64 && (vt & (vt - 1)) == 0 && (dv & (dv - 1)) == 0;
+  const int shuffles = vt <= 64 && (vt & (vt - 1)) == 0 && (UG ? (dv & (dv - 1)) == 0 : VEC % D == 0);
   const size_t lds = gn_fwd_lds(p.W, p.threads, VEC, D);
   if (int rc = gn_allow_lds(gn_resident_fwd_kernel<T, NV, UG, ACT>, lds)) return rc;
   hipLaunchKernelGGL((gn_resident_fwd_kernel<T, NV, UG, ACT>), dim3((unsigned)(a.N * (a.C / p.W))), dim3(p.threads), lds, a.st,
@@ -424,6 +523,7 @@ template <typename T, int NV, bool UG, int ACT> static int gn_launch_bwd(const G
 #define GN_RES_ACT(FN, NV, UG)                                                      \
   switch (a.act) {                                                                  \
     case GN_NONE: return FN<T, NV, UG, GN_NONE>(p, a);                              \
+    case GN_RELU: return FN<T, NV, UG, GN_RELU>(p, a);                              \
     case GN_CAP: return FN<T, NV, UG, GN_CAP>(p, a);                                \
     default: return FN<T, NV, UG, GN_SILU>(p, a);                                   \
   }
@@ -439,6 +539,7 @@ template <typename T> int gn_resident_fwd(const GnPlan& p, const GnResidentArgs&
 template <typename T> int gn_resident_bwd(const GnPlan& p, const GnResidentArgs& a) {
   if (p.nv <= 2) { GN_RES_UG(gn_launch_bwd, 2) }
   if (p.nv <= 4) { GN_RES_UG(gn_launch_bwd, 4) }
+  if (p.nv <= GN_NV_BOTH) { GN_RES_UG(gn_launch_bwd, GN_NV_BOTH) }
   GN_RES_UG(gn_launch_bwd, GN_NV_BWD)
 }
 #endif
