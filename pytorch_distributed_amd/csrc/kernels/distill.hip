@@ -46,6 +46,35 @@ __device__ __forceinline__ void ms_add(MaxSum& a, float z, float c) {
   }
   a.s += ms_exp(z, a.m, c);
 }
+// 2^x.  The hardware's own is enough for 16-bit logits; fp32 gradients may be denormal, which it flushes.
+template <typename T> __device__ __forceinline__ float fast_exp2(float x) {
+  return sizeof(T) == 4 ? exp2f(x) : __builtin_amdgcn_exp2f(x);
+}
+// The same running pair for whole vectors, on the scale that the exponential takes: sum of 2^(z*c - mc) with one
+// multiply-add an element.  mc is the rounded product of the maximum and c; flush() takes its rounding out of the sum.
+// A sum of 0 can also mean that every value is the lowest fp32 number: the caller looks again with ms_add then.
+struct FastSum {
+  float m = -FLT_MAX, mc = 0.f, s = 0.f;
+  __device__ __forceinline__ void raise(float m2, float c) {
+    const float mc2 = m2 * c;
+    s *= s == 0.f ? 0.f : __builtin_amdgcn_exp2f(mc - mc2);
+    m = m2;
+    mc = mc2;
+  }
+  template <typename T, int N> __device__ __forceinline__ void add(const float (&z)[N], float c) {
+    float top = z[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) top = fmaxf(top, z[e]);
+    if (top > m) raise(top, c);
+    float a = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) a += __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], c, -mc));
+    s += a;
+  }
+  __device__ __forceinline__ MaxSum flush(float c) const {
+    return MaxSum{m, s == 0.f ? 0.f : s * __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -mc))};
+  }
+};
 template <int NT>
 __device__ __forceinline__ MaxSum ms_block(MaxSum a, float c, float* scratch /* 2*NT/64 */) {
 #pragma unroll
@@ -107,29 +136,33 @@ __device__ __forceinline__ int radix_digit(unsigned* hist, int& need, bool ascen
   return out[0];
 }
 
-// One block a row.  The k-th largest key is found digit by digit (a histogram of 256 counts a pass over the row), then,
-// where more values equal it than are wanted, the highest class that still belongs, digit by digit of the class; the k
-// elements are gathered and ranked by counting.
+constexpr int MAX_CAND = 1536;  // elements that are ranked
+
+struct TopShared {
+  unsigned hist[256];
+  int pick[2];
+  int count;
+  unsigned long long cand[MAX_CAND];  // key, then the class from the last to the first: larger is better
+};
+__device__ __forceinline__ unsigned long long cand_of(unsigned key, int j) {
+  return ((unsigned long long)key << 32) | (0xffffffffu - (unsigned)j);
+}
+
+// For any row: the k-th largest key is found digit by digit (a histogram of 256 counts a pass over the row), then, where
+// more values equal it than are wanted, the highest class that still belongs, digit by digit of the class.  Leaves the K
+// elements in sh.cand and returns the pair of all others.
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT)
-top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, double temperature, T* __restrict__ values,
-                  long long* __restrict__ indices, float* __restrict__ rest) {
-  __shared__ unsigned hist[256];
-  __shared__ int pick[2];
-  __shared__ int count;
-  __shared__ float scratch[2 * NT / 64];
-  __shared__ unsigned long long cand[MAX_K];
-  const T* row = z + (long long)blockIdx.x * ld;
+__device__ MaxSum top_by_digits(const T* row, int V, int K, float c, TopShared& sh) {
   unsigned key = 0;
   int need = K;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += NT) hist[i] = 0;
+    for (int i = threadIdx.x; i < 256; i += NT) sh.hist[i] = 0;
     __syncthreads();
     for (int j = threadIdx.x; j < V; j += NT) {
       const unsigned q = order_key(ElemTraits<T>::to_f32(row[j]));
-      if (shift == 24 || (q >> (shift + 8)) == key) atomicAdd(&hist[(q >> shift) & 255], 1u);
+      if (shift == 24 || (q >> (shift + 8)) == key) atomicAdd(&sh.hist[(q >> shift) & 255], 1u);
     }
-    key = (key << 8) | (unsigned)radix_digit<NT>(hist, need, false, pick);
+    key = (key << 8) | (unsigned)radix_digit<NT>(sh.hist, need, false, sh.pick);
     __syncthreads();
   }
   // need of the elements that equal key are wanted, those of the lowest classes
@@ -137,37 +170,149 @@ top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, 
   int top_shift = 0;
   while (((V - 1) >> top_shift) > 255) top_shift += 8;
   for (int shift = top_shift; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += NT) hist[i] = 0;
+    for (int i = threadIdx.x; i < 256; i += NT) sh.hist[i] = 0;
     __syncthreads();
     for (int j = threadIdx.x; j < V; j += NT) {
       if (order_key(ElemTraits<T>::to_f32(row[j])) != key) continue;
-      if (shift == top_shift || ((unsigned)j >> (shift + 8)) == last) atomicAdd(&hist[((unsigned)j >> shift) & 255], 1u);
+      if (shift == top_shift || ((unsigned)j >> (shift + 8)) == last) atomicAdd(&sh.hist[((unsigned)j >> shift) & 255], 1u);
     }
-    last = (last << 8) | (unsigned)radix_digit<NT>(hist, need, true, pick);
+    last = (last << 8) | (unsigned)radix_digit<NT>(sh.hist, need, true, sh.pick);
     __syncthreads();
   }
-  if (threadIdx.x == 0) count = 0;
+  if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
   MaxSum ms{-FLT_MAX, 0.f};
   for (int j = threadIdx.x; j < V; j += NT) {
     const float v = ElemTraits<T>::to_f32(row[j]);
     const unsigned q = order_key(v);
     if (q > key || (q == key && (unsigned)j <= last)) {
-      const int p = atomicAdd(&count, 1);
-      if (p < MAX_K) cand[p] = ((unsigned long long)q << 32) | (0xffffffffu - (unsigned)j);
+      const int p = atomicAdd(&sh.count, 1);
+      if (p < MAX_CAND) sh.cand[p] = cand_of(q, j);
     } else {
       ms_add(ms, v, c);
     }
   }
-  ms = ms_block<NT>(ms, c, scratch);  // its barriers also close the list of candidates
-  for (int i = threadIdx.x; i < K; i += NT) {
-    const unsigned long long me = cand[i];
-    int r = 0;
-    for (int o = 0; o < K; ++o) r += cand[o] > me ? 1 : 0;
-    const unsigned j = 0xffffffffu - (unsigned)me;
-    values[(long long)blockIdx.x * K + r] = row[j];
-    indices[(long long)blockIdx.x * K + r] = (long long)j;
+  __syncthreads();
+  return ms;
+}
+
+// One block a row, one read of it from memory.  A thread's vectors are cut into CELLS runs; of each run it keeps the
+// maximum and the sum of exponentials.  The K-th largest of the threads' maxima is a bound that at least K elements reach,
+// and not many more do: only the runs that reach it are read again (from the caches), their elements at or above the bound
+// become candidates, and the K best are found by counting for each candidate how many are better.  The log-sum-exp of the
+// others is joined from the runs without a candidate and the single elements of the others, nothing is taken off a sum.
+// Rows that do not fit this (more candidates than MAX_CAND: many equal values, K near the number of threads) go digit by digit.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT)
+top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, double temperature, T* __restrict__ values,
+                  long long* __restrict__ indices, float* __restrict__ rest) {
+  constexpr int CELLS = 16, VN = RowVec<T>::N;
+  __shared__ TopShared sh;
+  __shared__ float scratch[2 * NT / 64];
+  const T* row = z + (long long)blockIdx.x * ld;
+  const int nv = (V + VN - 1) / VN;              // the last vector may be short
+  const int per = (nv + CELLS * NT - 1) / (CELLS * NT);  // vectors of a run: thread + NT*(run*per + 0 .. per-1)
+  const auto fetch = [&](int i, float (&zf)[VN]) {
+    if ((i + 1) * VN <= V) {
+      const RowVec<T> v = row_ld(row + (long long)i * VN);
+#pragma unroll
+      for (int e = 0; e < VN; ++e) zf[e] = ElemTraits<T>::to_f32(v.v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VN; ++e) zf[e] = i * VN + e < V ? ElemTraits<T>::to_f32(row[i * VN + e]) : -INFINITY;
+    }
+  };
+  MaxSum cell[CELLS];
+  float most = -INFINITY;
+#pragma unroll
+  for (int q = 0; q < CELLS; ++q) {
+    FastSum fs;
+    for (int p = 0; p < per; ++p) {
+      const int i = threadIdx.x + NT * (q * per + p);
+      if (i < nv) {
+        float zf[VN];
+        fetch(i, zf);
+        fs.add<T>(zf, c);
+      }
+    }
+    cell[q] = fs.flush(c);
+    most = cell[q].s == 0.f ? most : fmaxf(most, cell[q].m);
   }
+  for (int i = threadIdx.x; i < 256; i += NT) sh.hist[i] = 0;
+  if (threadIdx.x == 0) sh.count = 0;
+  // a NaN or +inf leaves a sum that is no number: such a thread looks for its maximum again
+  bool odd = false;
+#pragma unroll
+  for (int q = 0; q < CELLS; ++q) odd |= !(cell[q].s < INFINITY);
+  unsigned mine = order_key(most);
+  if (odd) {
+    mine = 0;
+    for (int i = threadIdx.x; i < nv; i += NT)
+      for (int e = 0; e < VN && i * VN + e < V; ++e) mine = max(mine, order_key(ElemTraits<T>::to_f32(row[i * VN + e])));
+  }
+  // the bound, to the upper 16 bits of the key
+  bool fits = K <= NT;
+  unsigned bound = 0;
+  if (fits) {
+    int need = K;
+    __syncthreads();
+    atomicAdd(&sh.hist[mine >> 24], 1u);
+    bound = (unsigned)radix_digit<NT>(sh.hist, need, false, sh.pick);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256; i += NT) sh.hist[i] = 0;
+    __syncthreads();
+    if (mine >> 24 == bound) atomicAdd(&sh.hist[(mine >> 16) & 255], 1u);
+    bound = ((bound << 8) | (unsigned)radix_digit<NT>(sh.hist, need, false, sh.pick)) << 16;
+  }
+  MaxSum ms{-FLT_MAX, 0.f};
+  if (fits) {
+#pragma unroll
+    for (int q = 0; q < CELLS; ++q) {
+      // (a sum of 0: infinities below, or the lowest fp32 number)
+      const bool again = !(cell[q].s < INFINITY) || cell[q].s == 0.f || order_key(cell[q].m) >= bound;
+      if (!again) {
+        ms_merge(ms, cell[q].m, cell[q].s, c);
+        continue;
+      }
+      for (int p = 0; p < per; ++p) {
+        const int i = threadIdx.x + NT * (q * per + p);
+        if (i >= nv) break;
+        float zf[VN];
+        fetch(i, zf);
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          if (i * VN + e >= V) continue;
+          const unsigned key = order_key(zf[e]);
+          if (key >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < MAX_CAND) sh.cand[at] = cand_of(key, i * VN + e);
+          } else {
+            ms_add(ms, zf[e], c);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    fits = sh.count >= K && sh.count <= MAX_CAND;
+  }
+  if (!fits) {
+    __syncthreads();
+    ms = top_by_digits<T, NT>(row, V, K, c, sh);
+  }
+  const int n = sh.count;
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const unsigned long long me = sh.cand[i];
+    int r = 0;
+    for (int o = 0; o < n; ++o) r += sh.cand[o] > me ? 1 : 0;
+    const unsigned j = 0xffffffffu - (unsigned)me;
+    if (r < K) {
+      values[(long long)blockIdx.x * K + r] = row[j];
+      indices[(long long)blockIdx.x * K + r] = (long long)j;
+    } else {
+      ms_add(ms, ElemTraits<T>::to_f32(row[j]), c);
+    }
+  }
+  ms = ms_block<NT>(ms, c, scratch);
   if (threadIdx.x == 0)
     rest[blockIdx.x] = ms.s == 0.f ? -INFINITY : (float)((double)ms.m / temperature + log((double)ms.s));
 }
@@ -245,20 +390,43 @@ distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
     }
   }
   __syncthreads();
-  MaxSum ms{-FLT_MAX, 0.f};
   const int nv = V / VN;
   const unsigned char* bytes = reinterpret_cast<const unsigned char*>(en.bits);
-  for (int i = threadIdx.x; i < nv; i += NT) {
-    const RowVec<T> v = row_ld(row + (long long)i * VN);
-    unsigned skip = 0;
-    if (rest) skip = VN == 8 ? bytes[i] : (bytes[i >> 1] >> ((i & 1) * 4)) & 15u;
+  const auto fetch = [&](int i) { return row_ld(row + (long long)i * VN); };
+  FastSum fs;
+  const auto take = [&](const RowVec<T>& v, int i) {
+    float zf[VN];
 #pragma unroll
-    for (int e = 0; e < VN; ++e)
-      if (!((skip >> e) & 1u)) ms_add(ms, ElemTraits<T>::to_f32(v.v[e]), c);
+    for (int e = 0; e < VN; ++e) zf[e] = ElemTraits<T>::to_f32(v.v[e]);
+    if (rest) {
+      const unsigned skip = VN == 8 ? bytes[i] : (bytes[i >> 1] >> ((i & 1) * 4)) & 15u;
+      if (skip)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) zf[e] = (skip >> e) & 1u ? -INFINITY : zf[e];
+    }
+    fs.add<T>(zf, c);
+  };
+  constexpr int U = 4;  // loads in flight
+  int i = threadIdx.x;
+  for (; i + (U - 1) * NT < nv; i += U * NT) {
+    RowVec<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = fetch(i + u * NT);
+#pragma unroll
+    for (int u = 0; u < U; ++u) take(v[u], i + u * NT);
   }
+  for (; i < nv; i += NT) take(fetch(i), i);
+  MaxSum ms = fs.flush(c);
+  const auto skipped = [&](int j) { return rest && ((en.bits[j >> 5] >> (j & 31)) & 1u); };
   for (int j = nv * VN + threadIdx.x; j < V; j += NT)
-    if (!rest || !((en.bits[j >> 5] >> (j & 31)) & 1u)) ms_add(ms, ElemTraits<T>::to_f32(row[j]), c);
+    if (!skipped(j)) ms_add(ms, ElemTraits<T>::to_f32(row[j]), c);
   ms = ms_block<NT>(ms, c, scratch);
+  if (ms.s == 0.f) {  // nothing above the lowest number
+    ms = MaxSum{-FLT_MAX, 0.f};
+    for (int j = threadIdx.x; j < V; j += NT)
+      if (!skipped(j)) ms_add(ms, ElemTraits<T>::to_f32(row[j]), c);
+    ms = ms_block<NT>(ms, c, scratch);
+  }
   if (twice)  // rare: entries of one class are one class of the distribution
     for (int k = threadIdx.x; k < K; k += NT)
       if (en.idx[k] >= 0)
@@ -349,12 +517,13 @@ distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
 }
 
 // dz of a row: one value for every class, then the entries' own over it (the barrier orders the two writes).
+// Rows go from the last to the first: what the forward pass read last is still in the memory-side cache.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT)
 distill_bwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __restrict__ indices, int idx64, long long ild,
                    int K, float c, const RowStat* __restrict__ stat, const float* __restrict__ dtop,
                    const float* __restrict__ g, int gstride, float gscale, T* __restrict__ dz) {
-  const long long rowi = blockIdx.x;
+  const long long rowi = gridDim.x - 1 - blockIdx.x;
   const T* row = z + rowi * ld;
   T* out = dz + rowi * V;
   constexpr int VN = RowVec<T>::N;
@@ -369,15 +538,26 @@ distill_bwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
     for (int i = threadIdx.x; i < nv; i += NT) row_st(out + (long long)i * VN, v);
     for (int j = nv * VN + threadIdx.x; j < V; j += NT) out[j] = ElemTraits<T>::from_f32(0.f);
   } else {
-    for (int i = threadIdx.x; i < nv; i += NT) {
-      RowVec<T> v = row_ld(row + (long long)i * VN);
+    const auto value = [&](float zf) { return fast_exp2<T>((zf - st.shift) * c) * f; };
+    const auto put = [&](RowVec<T>& v, int i) {
 #pragma unroll
-      for (int e = 0; e < VN; ++e)
-        v.v[e] = ElemTraits<T>::from_f32(exp2f((ElemTraits<T>::to_f32(v.v[e]) - st.shift) * c) * f);
+      for (int e = 0; e < VN; ++e) v.v[e] = ElemTraits<T>::from_f32(value(ElemTraits<T>::to_f32(v.v[e])));
       row_st(out + (long long)i * VN, v);
+    };
+    constexpr int U = 4;
+    int i = threadIdx.x;
+    for (; i + (U - 1) * NT < nv; i += U * NT) {
+      RowVec<T> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = row_ld(row + (long long)(i + u * NT) * VN);
+#pragma unroll
+      for (int u = 0; u < U; ++u) put(v[u], i + u * NT);
     }
-    for (int j = nv * VN + threadIdx.x; j < V; j += NT)
-      out[j] = ElemTraits<T>::from_f32(exp2f((ElemTraits<T>::to_f32(row[j]) - st.shift) * c) * f);
+    for (; i < nv; i += NT) {
+      RowVec<T> v = row_ld(row + (long long)i * VN);
+      put(v, i);
+    }
+    for (int j = nv * VN + threadIdx.x; j < V; j += NT) out[j] = ElemTraits<T>::from_f32(value(ElemTraits<T>::to_f32(row[j])));
   }
   __syncthreads();
   for (int k = threadIdx.x; k < K; k += NT) {
@@ -417,8 +597,13 @@ PDA_EXPORT int pda_top_logits(int dtype, const void* z, long long ld, long long 
                               void* values, long long* indices, float* rest, hipStream_t st) {
   if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || K <= 0 || K > V || K > MAX_K || !(temperature > 0.0)) return -1;
   const float c = (float)(LOG2E / temperature);
-  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, (const T*)z,
-                                             ld, V, K, c, temperature, (T*)values, indices, rest));
+  // rows of up to 32 KB: a run of one or two vectors with 256 threads; longer ones get 512
+  if ((long long)V * (dtype == PDA_F32 ? 4 : 2) <= 32 * 1024)
+    DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, (const T*)z,
+                                               ld, V, K, c, temperature, (T*)values, indices, rest))
+  else
+    DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, 512>), dim3((unsigned)rows), dim3(512), 0, st, (const T*)z,
+                                               ld, V, K, c, temperature, (T*)values, indices, rest))
   return pda_check_launch();
 }
 
