@@ -61,7 +61,7 @@ struct FastSum {
     m = m2;
     mc = mc2;
   }
-  template <typename T, int N> __device__ __forceinline__ void add(const float (&z)[N], float c) {
+  template <int N> __device__ __forceinline__ void add(const float (&z)[N], float c) {
     float top = z[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, z[e]);
@@ -202,41 +202,43 @@ __device__ MaxSum top_by_digits(const T* row, int V, int K, float c, TopShared& 
 // become candidates, and the K best are found by counting for each candidate how many are better.  The log-sum-exp of the
 // others is joined from the runs without a candidate and the single elements of the others, nothing is taken off a sum.
 // Rows that do not fit this (more candidates than MAX_CAND: many equal values, K near the number of threads) go digit by digit.
-template <typename T, int NT>
+template <typename T, int NT, int CELLS>
 __global__ void __launch_bounds__(NT)
 top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, double temperature, T* __restrict__ values,
                   long long* __restrict__ indices, float* __restrict__ rest) {
-  constexpr int CELLS = 16, VN = RowVec<T>::N;
+  constexpr int VN = RowVec<T>::N, U = CELLS < 8 ? CELLS : 8;  // U: loads in flight
+  constexpr int NM = CELLS * (NT / 64);                            // one mask of lanes a run and wave
   __shared__ TopShared sh;
+  __shared__ int before[NM + 1];
+  __shared__ unsigned short queue[CELLS * NT];
   __shared__ float scratch[2 * NT / 64];
   const T* row = z + (long long)blockIdx.x * ld;
-  const int nv = (V + VN - 1) / VN;              // the last vector may be short
+  const int nv = V / VN;                                 // whole vectors; a thread each takes what is left
   const int per = (nv + CELLS * NT - 1) / (CELLS * NT);  // vectors of a run: thread + NT*(run*per + 0 .. per-1)
-  const auto fetch = [&](int i, float (&zf)[VN]) {
-    if ((i + 1) * VN <= V) {
-      const RowVec<T> v = row_ld(row + (long long)i * VN);
-#pragma unroll
-      for (int e = 0; e < VN; ++e) zf[e] = ElemTraits<T>::to_f32(v.v[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VN; ++e) zf[e] = i * VN + e < V ? ElemTraits<T>::to_f32(row[i * VN + e]) : -INFINITY;
-    }
-  };
+  const int extra = nv * VN + threadIdx.x;
   MaxSum cell[CELLS];
   float most = -INFINITY;
 #pragma unroll
-  for (int q = 0; q < CELLS; ++q) {
-    FastSum fs;
+  for (int q0 = 0; q0 < CELLS; q0 += U) {
+    FastSum fs[U];
     for (int p = 0; p < per; ++p) {
-      const int i = threadIdx.x + NT * (q * per + p);
-      if (i < nv) {
-        float zf[VN];
-        fetch(i, zf);
-        fs.add<T>(zf, c);
-      }
+      RowVec<T> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = row_ld(row + (long long)min(threadIdx.x + NT * ((q0 + u) * per + p), nv - 1) * VN);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if ((int)threadIdx.x + NT * ((q0 + u) * per + p) < nv) {
+          float zf[VN];
+#pragma unroll
+          for (int e = 0; e < VN; ++e) zf[e] = ElemTraits<T>::to_f32(v[u].v[e]);
+          fs[u].add(zf, c);
+        }
     }
-    cell[q] = fs.flush(c);
-    most = cell[q].s == 0.f ? most : fmaxf(most, cell[q].m);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      cell[q0 + u] = fs[u].flush(c);
+      most = cell[q0 + u].s == 0.f ? most : fmaxf(most, cell[q0 + u].m);
+    }
   }
   for (int i = threadIdx.x; i < 256; i += NT) sh.hist[i] = 0;
   if (threadIdx.x == 0) sh.count = 0;
@@ -248,8 +250,9 @@ top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, 
   if (odd) {
     mine = 0;
     for (int i = threadIdx.x; i < nv; i += NT)
-      for (int e = 0; e < VN && i * VN + e < V; ++e) mine = max(mine, order_key(ElemTraits<T>::to_f32(row[i * VN + e])));
+      for (int e = 0; e < VN; ++e) mine = max(mine, order_key(ElemTraits<T>::to_f32(row[i * VN + e])));
   }
+  if (extra < V) mine = max(mine, order_key(ElemTraits<T>::to_f32(row[extra])));
   // the bound, to the upper 16 bits of the key
   bool fits = K <= NT;
   unsigned bound = 0;
@@ -265,33 +268,67 @@ top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, 
     bound = ((bound << 8) | (unsigned)radix_digit<NT>(sh.hist, need, false, sh.pick)) << 16;
   }
   MaxSum ms{-FLT_MAX, 0.f};
+  const auto one = [&](float v, int j) {
+    const unsigned key = order_key(v);
+    if (key >= bound) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < MAX_CAND) sh.cand[at] = cand_of(key, j);
+    } else {
+      ms_add(ms, v, c);
+    }
+  };
   if (fits) {
+    // the runs to read again, as a list in the order of run and thread: all their vectors are then fetched at once
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    unsigned long long mask[CELLS];
 #pragma unroll
     for (int q = 0; q < CELLS; ++q) {
       // (a sum of 0: infinities below, or the lowest fp32 number)
-      const bool again = !(cell[q].s < INFINITY) || cell[q].s == 0.f || order_key(cell[q].m) >= bound;
-      if (!again) {
-        ms_merge(ms, cell[q].m, cell[q].s, c);
-        continue;
-      }
-      for (int p = 0; p < per; ++p) {
-        const int i = threadIdx.x + NT * (q * per + p);
-        if (i >= nv) break;
-        float zf[VN];
-        fetch(i, zf);
+      const bool some = (int)threadIdx.x + NT * q * per < nv;
+      const bool again = some && (!(cell[q].s < INFINITY) || cell[q].s == 0.f || order_key(cell[q].m) >= bound);
+      mask[q] = __ballot(again);
+      if (lane == 0) before[q * (NT / 64) + wave] = __popcll(mask[q]);
+      if (some && !again) ms_merge(ms, cell[q].m, cell[q].s, c);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      int own = 0;
+      constexpr int PER = (NM + 63) / 64;
+      int n[PER];
 #pragma unroll
-        for (int e = 0; e < VN; ++e) {
-          if (i * VN + e >= V) continue;
-          const unsigned key = order_key(zf[e]);
-          if (key >= bound) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < MAX_CAND) sh.cand[at] = cand_of(key, i * VN + e);
-          } else {
-            ms_add(ms, zf[e], c);
-          }
-        }
+      for (int i = 0; i < PER; ++i) {
+        n[i] = lane * PER + i < NM ? before[lane * PER + i] : 0;
+        own += n[i];
+      }
+      int sum = own;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += t;
+      }
+      if (lane == 63) before[NM] = sum;
+      sum -= own;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (lane * PER + i < NM) before[lane * PER + i] = sum;
+        sum += n[i];
       }
     }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < CELLS; ++q)
+      if ((mask[q] >> lane) & 1ull)
+        queue[before[q * (NT / 64) + wave] + __popcll(mask[q] & ((1ull << lane) - 1ull))] = (unsigned short)(q * NT + threadIdx.x);
+    __syncthreads();
+    const int todo = before[NM] * per;
+    for (int w = threadIdx.x; w < todo; w += NT) {
+      const int e0 = queue[w / per], i = (e0 % NT) + NT * ((e0 / NT) * per + w % per);
+      if (i >= nv) continue;
+      const RowVec<T> v = row_ld(row + (long long)i * VN);
+#pragma unroll
+      for (int e = 0; e < VN; ++e) one(ElemTraits<T>::to_f32(v.v[e]), i * VN + e);
+    }
+    if (extra < V) one(ElemTraits<T>::to_f32(row[extra]), extra);
     __syncthreads();
     fits = sh.count >= K && sh.count <= MAX_CAND;
   }
@@ -299,15 +336,31 @@ top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, 
     __syncthreads();
     ms = top_by_digits<T, NT>(row, V, K, c, sh);
   }
+  // in order of rank (the list's own order is that of the atomics): what comes after the K-th joins the others
   const int n = sh.count;
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const unsigned long long me = sh.cand[i];
+  constexpr int PER = (MAX_CAND + NT - 1) / NT;
+  unsigned long long me[PER];
+  int rank[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int i = threadIdx.x + p * NT;
+    rank[p] = -1;
+    if (i >= n) continue;
+    me[p] = sh.cand[i];
     int r = 0;
-    for (int o = 0; o < n; ++o) r += sh.cand[o] > me ? 1 : 0;
-    const unsigned j = 0xffffffffu - (unsigned)me;
-    if (r < K) {
-      values[(long long)blockIdx.x * K + r] = row[j];
-      indices[(long long)blockIdx.x * K + r] = (long long)j;
+    for (int o = 0; o < n; ++o) r += sh.cand[o] > me[p] ? 1 : 0;
+    rank[p] = r;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < PER; ++p)
+    if (rank[p] >= 0) sh.cand[rank[p]] = me[p];
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const unsigned j = 0xffffffffu - (unsigned)sh.cand[i];
+    if (i < K) {
+      values[(long long)blockIdx.x * K + i] = row[j];
+      indices[(long long)blockIdx.x * K + i] = (long long)j;
     } else {
       ms_add(ms, ElemTraits<T>::to_f32(row[j]), c);
     }
@@ -404,7 +457,7 @@ distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
 #pragma unroll
         for (int e = 0; e < VN; ++e) zf[e] = (skip >> e) & 1u ? -INFINITY : zf[e];
     }
-    fs.add<T>(zf, c);
+    fs.add(zf, c);
   };
   constexpr int U = 4;  // loads in flight
   int i = threadIdx.x;
@@ -597,13 +650,18 @@ PDA_EXPORT int pda_top_logits(int dtype, const void* z, long long ld, long long 
                               void* values, long long* indices, float* rest, hipStream_t st) {
   if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || K <= 0 || K > V || K > MAX_K || !(temperature > 0.0)) return -1;
   const float c = (float)(LOG2E / temperature);
-  // rows of up to 32 KB: a run of one or two vectors with 256 threads; longer ones get 512
-  if ((long long)V * (dtype == PDA_F32 ? 4 : 2) <= 32 * 1024)
-    DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, (const T*)z,
-                                               ld, V, K, c, temperature, (T*)values, indices, rest))
-  else
-    DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, 512>), dim3((unsigned)rows), dim3(512), 0, st, (const T*)z,
-                                               ld, V, K, c, temperature, (T*)values, indices, rest))
+  // short rows: no more runs than they have vectors; above 32 KB twice the threads
+  const long long bytes = (long long)V * (dtype == PDA_F32 ? 4 : 2);
+#define TOP_LAUNCH(NT, CELLS)                                                                                                  \
+  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, NT, CELLS>), dim3((unsigned)rows), dim3(NT), 0, st,           \
+                                             (const T*)z, ld, V, K, c, temperature, (T*)values, indices, rest))
+  if (bytes <= 8 * 1024) {
+    TOP_LAUNCH(256, 2)
+  } else if (bytes <= 32 * 1024) {
+    TOP_LAUNCH(256, 8)
+  } else {
+    TOP_LAUNCH(512, 16)
+  }
   return pda_check_launch();
 }
 

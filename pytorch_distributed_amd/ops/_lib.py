@@ -7,6 +7,7 @@ reference path in this package exists only for tensors that live on the CPU.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -181,6 +182,17 @@ def stream():
     if _RAW_STREAM is not None and _GET_DEVICE is not None:
         return _RAW_STREAM(_GET_DEVICE())
     return torch.cuda.current_stream().cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (and :func:`stream` is its current stream); free of cost where it
+    is already."""
+    if _GET_DEVICE is not None and _GET_DEVICE() == t.get_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(t.device)
 
 
 def check(rc: int, name: str) -> None:

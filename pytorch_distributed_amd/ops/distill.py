@@ -29,8 +29,8 @@ def _temperature(t) -> float:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``[rows, last]`` view (a copy only where the last dimension is strided or the leading ones do not collapse)."""
-    r = t.reshape(-1, t.shape[-1])
-    return r if r.shape[-1] <= 1 or r.stride(-1) == 1 else r.contiguous()
+    r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return r if r.shape[1] <= 1 or r.stride(1) == 1 else r.contiguous()
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -57,7 +57,6 @@ def top_logits_ref(logits, k, temperature):
     return logits.gather(-1, idx), idx, rest
 
 
-@torch.no_grad()
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(values, indices, rest)`` of the ``k`` largest of every row of ``logits`` (``[..., classes]``).
 
@@ -71,14 +70,15 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> Tuple[
     if not 1 <= k <= min(V, MAX_K):
         raise ValueError(f"top_logits: k = {k} of {V} classes; 1 to {min(V, MAX_K)} are supported")
     if not logits.is_cuda or logits.numel() == 0:
-        return top_logits_ref(logits, k, t)
+        with torch.no_grad():
+            return top_logits_ref(logits, k, t)
     l = _lib.lib()
-    z = _rows(logits.detach())
+    z = _rows(logits.detach() if logits.requires_grad else logits)
     lead = logits.shape[:-1]
     values = torch.empty(lead + (k,), device=z.device, dtype=z.dtype)
     indices = torch.empty(lead + (k,), device=z.device, dtype=torch.int64)
     rest = torch.empty(lead, device=z.device, dtype=torch.float32)
-    with torch.cuda.device(z.device):
+    with _lib.on_device_of(z):
         _lib.check(l.pda_top_logits(_lib.dt(z), z.data_ptr(), _row_stride(z), z.shape[0], V, k, t, values.data_ptr(),
                                     indices.data_ptr(), rest.data_ptr(), _lib.stream()), "pda_top_logits")
     return values, indices, rest
@@ -89,39 +89,50 @@ class _DistillFn(torch.autograd.Function):
     def forward(ctx, logits, values, indices, rest, temperature, reduction):
         l = _lib.lib()
         z, v, i = _rows(logits), _rows(values), _rows(indices)
-        rest = None if rest is None else rest.reshape(-1).float().contiguous()
+        if rest is not None:
+            rest = rest.reshape(-1).float().contiguous()
         (rows, V), K = z.shape, v.shape[1]
-        dev = z.device
-        with torch.cuda.device(dev):
-            row_loss = torch.empty((rows,), device=dev, dtype=torch.float32)
-            stat = torch.empty((rows, 2), device=dev, dtype=torch.float32)
-            dtop = torch.empty((rows, K), device=dev, dtype=torch.float32)
-            loss = None if reduction == "none" else torch.empty((), device=dev, dtype=torch.float32)
-            _lib.check(l.pda_distill_fwd(_lib.dt(z), z.data_ptr(), _row_stride(z), rows, V, v.data_ptr(), _lib.dt(v),
-                                         _row_stride(v), i.data_ptr(), int(i.dtype == torch.int64), _row_stride(i),
-                                         _lib.ptr(rest), K, temperature, row_loss.data_ptr(), stat.data_ptr(),
-                                         dtop.data_ptr(), _lib.ptr(loss), 1.0 / rows if reduction == "mean" else 1.0,
-                                         _lib.stream()), "pda_distill_fwd")
-        ctx.save_for_backward(z, i, stat, dtop)
+        code, i64 = _lib.dt(z), int(i.dtype is torch.int64)
+        with _lib.on_device_of(z):
+            # what the rows leave for the backward pass: a shift and a factor each, then one number an entry
+            left = torch.empty((rows, 2 + K), device=z.device, dtype=torch.float32)
+            row_loss = torch.empty((rows,), device=z.device, dtype=torch.float32)
+            loss = None if reduction == "none" else torch.empty((), device=z.device, dtype=torch.float32)
+            at = left.data_ptr()
+            _lib.check(l.pda_distill_fwd(code, z.data_ptr(), _row_stride(z), rows, V, v.data_ptr(), _lib.dt(v), _row_stride(v),
+                                         i.data_ptr(), i64, _row_stride(i), _lib.ptr(rest), K, temperature,
+                                         row_loss.data_ptr(), at, at + 8 * rows, _lib.ptr(loss),
+                                         1.0 / rows if reduction == "mean" else 1.0, _lib.stream()), "pda_distill_fwd")
+        ctx.save_for_backward(z, i, left)
         ctx.cfg = (logits.shape, temperature, reduction)
-        return row_loss.view(logits.shape[:-1]) if loss is None else loss
+        if loss is not None:
+            return loss
+        return row_loss if logits.dim() == 2 else row_loss.view(logits.shape[:-1])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        l = _lib.lib()
-        z, i, stat, dtop = ctx.saved_tensors
-        shape, temperature, reduction = ctx.cfg
-        rows, V = z.shape
-        g = g.reshape(-1).float().contiguous()
-        scale = temperature / rows if reduction == "mean" else temperature
-        with torch.cuda.device(z.device):
-            dz = torch.empty((rows, V), device=z.device, dtype=z.dtype)
-            _lib.check(l.pda_distill_bwd(_lib.dt(z), z.data_ptr(), _row_stride(z), rows, V, i.data_ptr(),
-                                         int(i.dtype == torch.int64), _row_stride(i), i.shape[1], temperature,
-                                         stat.data_ptr(), dtop.data_ptr(), g.data_ptr(), int(reduction == "none"), scale,
-                                         dz.data_ptr(), _lib.stream()), "pda_distill_bwd")
-        return dz.view(shape), None, None, None, None, None
+        return _backward_once(ctx, g) if torch.is_grad_enabled() else _backward(ctx, g)
+
+
+def _backward(ctx, g):
+    l = _lib.lib()
+    z, i, left = ctx.saved_tensors
+    shape, temperature, reduction = ctx.cfg
+    rows, V = z.shape
+    if g.dtype is not torch.float32 or not g.is_contiguous():
+        g = g.float().contiguous()
+    with _lib.on_device_of(z):
+        dz = torch.empty((rows, V), device=z.device, dtype=z.dtype)
+        at = left.data_ptr()
+        _lib.check(l.pda_distill_bwd(_lib.dt(z), z.data_ptr(), _row_stride(z), rows, V, i.data_ptr(), int(i.dtype is torch.int64),
+                                     _row_stride(i), i.shape[1], temperature, at, at + 8 * rows, g.data_ptr(),
+                                     int(reduction == "none"), temperature / rows if reduction == "mean" else temperature,
+                                     dz.data_ptr(), _lib.stream()), "pda_distill_bwd")
+    return dz if len(shape) == 2 else dz.view(shape), None, None, None, None, None
+
+
+# under create_graph: the gradient is marked as not differentiable again
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def distill_loss_ref(logits, values, indices, rest, temperature, reduction):
@@ -190,10 +201,10 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_indices: to
         raise TypeError(f"distill_loss: top_indices must be int64 or int32, not {top_indices.dtype}")
     if rest is not None and (rest.shape != lead or rest.dtype not in _FLOATS):
         raise ValueError(f"distill_loss: rest must be floating-point numbers of shape {tuple(lead)}")
+    device = logits.device
     for name, x in (("top_values", top_values), ("top_indices", top_indices), ("rest", rest)):
-        if x is not None and x.device != logits.device:
-            raise ValueError(f"distill_loss: {name} is on {x.device}, logits on {logits.device}")
-    top_values, rest = top_values.detach(), None if rest is None else rest.detach()
+        if x is not None and x.device != device:
+            raise ValueError(f"distill_loss: {name} is on {x.device}, logits on {device}")
     if not logits.is_cuda or logits.numel() == 0:
-        return distill_loss_ref(logits, top_values, top_indices, rest, t, reduction)
+        return distill_loss_ref(logits, top_values.detach(), top_indices, None if rest is None else rest.detach(), t, reduction)
     return _DistillFn.apply(logits, top_values, top_indices, rest, t, reduction)

@@ -32,41 +32,43 @@ def _act_code(act) -> tuple:
 
 
 def _check(x, num_groups, gamma, beta, residual, eps) -> int:
-    if x.dim() < 2:
+    shape = x.shape
+    if len(shape) < 2:
         raise ValueError("group_norm_act: x must be [N, ..., C]")
     if x.dtype not in _FLOATS:
         raise TypeError(f"group_norm_act: unsupported dtype {x.dtype}")
-    C = x.shape[-1]
+    C = shape[-1]
     groups = int(num_groups)
     if groups <= 0 or C == 0 or C % groups != 0:
         raise ValueError(f"group_norm_act: {C} channels do not divide into {num_groups} groups")
-    if not float(eps) >= 0.0:
+    if not eps >= 0.0:
         raise ValueError("group_norm_act: eps must not be negative")
-    if (gamma is None) != (beta is None):
-        raise ValueError("group_norm_act: gamma and beta go together")
-    for name, t in (("gamma", gamma), ("beta", beta)):
-        if t is None:
-            continue
-        if t.shape != (C,) or t.dtype not in _FLOATS:
-            raise ValueError(f"group_norm_act: {name} must be {C} floating-point numbers")
-        if t.device != x.device:
-            raise ValueError(f"group_norm_act: {name} is on {t.device}, x on {x.device}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+    if gamma is not None or beta is not None:
+        if gamma is None or beta is None:
+            raise ValueError("group_norm_act: gamma and beta go together")
+        for name, t in (("gamma", gamma), ("beta", beta)):
+            if t.shape != (C,) or t.dtype not in _FLOATS:
+                raise ValueError(f"group_norm_act: {name} must be {C} floating-point numbers")
+            if t.device != x.device:
+                raise ValueError(f"group_norm_act: {name} is on {t.device}, x on {x.device}")
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("group_norm_act: residual must have x's shape, dtype and device")
     return groups
 
 
-def _plan(l, x, S: int, groups: int, backward: bool, *others) -> int:
+def _f32(p):
+    if p is None or (p.dtype is torch.float32 and p.is_contiguous()):
+        return p
+    return p.detach().float().contiguous()
+
+
+def _plan(l, code: int, N: int, S: int, C: int, groups: int, backward: int, *tensors) -> int:
     """0: a sample's groups stay in registers; otherwise the row chunks of the multi-pass kernels."""
-    aligned = all(t is None or t.data_ptr() % 16 == 0 for t in (x,) + others)
-    chunks = l.pda_group_norm_plan(_lib.dt(x), x.shape[0], S, x.shape[-1], groups, int(backward), int(aligned))
+    aligned = all(t is None or t.data_ptr() % 16 == 0 for t in tensors)
+    chunks = l.pda_group_norm_plan(code, N, S, C, groups, backward, int(aligned))
     if chunks < 0:
         _lib.check(chunks, "pda_group_norm_plan")
     return chunks
-
-
-def _f32(p):
-    return None if p is None else p.detach().float().contiguous()
 
 
 class _GroupNormActFn(torch.autograd.Function):
@@ -74,55 +76,66 @@ class _GroupNormActFn(torch.autograd.Function):
     def forward(ctx, x, gamma, beta, residual, groups, act, cap, eps):
         l = _lib.lib()
         x = x.contiguous()
-        residual = None if residual is None else residual.contiguous()
+        if residual is not None:
+            residual = residual.contiguous()
         N, C = x.shape[0], x.shape[-1]
         S = x.numel() // (N * C)
+        code = _lib.dt(x)
         out = torch.empty_like(x)
         ga, be = _f32(gamma), _f32(beta)
-        with torch.cuda.device(x.device):
-            chunks = _plan(l, x, S, groups, False, residual)
+        with _lib.on_device_of(x):
+            chunks = _plan(l, code, N, S, C, groups, 0, x, residual)
             part = torch.empty((N * chunks, C, 2), device=x.device, dtype=torch.float64) if chunks else None
             stats = torch.empty((N, groups, 2), device=x.device, dtype=torch.float64)
-            _lib.check(l.pda_group_norm_fwd(_lib.dt(x), x.data_ptr(), _lib.ptr(residual), out.data_ptr(), _lib.ptr(ga),
-                                            _lib.ptr(be), N, S, C, groups, eps, act, cap, chunks, _lib.ptr(part),
-                                            stats.data_ptr(), _lib.stream()), "pda_group_norm_fwd")
-        ctx.cfg = (groups, act, cap)
+            _lib.check(l.pda_group_norm_fwd(code, x.data_ptr(), _lib.ptr(residual), out.data_ptr(), _lib.ptr(ga), _lib.ptr(be),
+                                            N, S, C, groups, eps, act, cap, chunks, _lib.ptr(part), stats.data_ptr(),
+                                            _lib.stream()), "pda_group_norm_fwd")
+        ctx.cfg = (N, S, C, groups, act, cap)
         # with no activation the residual passes its gradient on unread
         ctx.save_for_backward(x, gamma, beta, residual if act else None, stats)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        l = _lib.lib()
-        x, gamma, beta, residual, stats = ctx.saved_tensors
-        groups, act, cap = ctx.cfg
-        dout = dout.contiguous()
-        N, C = x.shape[0], x.shape[-1]
-        S = x.numel() // (N * C)
-        want_dx, want_g, want_b, want_res = ctx.needs_input_grad[:4]
+        return _backward_once(ctx, dout) if torch.is_grad_enabled() else _backward(ctx, dout)
+
+
+def _backward(ctx, dout):
+    l = _lib.lib()
+    x, gamma, beta, residual, stats = ctx.saved_tensors
+    N, S, C, groups, act, cap = ctx.cfg
+    dout = dout.contiguous()
+    want_dx, want_g, want_b, want_res = ctx.needs_input_grad[:4]
+    dres = dx = dg = db = None
+    if want_res:
+        dres = torch.empty_like(x) if act else dout
+    if want_dx or (want_res and act):
+        dx = torch.empty_like(x)
+    params = want_g or want_b
+    if dx is not None or params:
+        code = _lib.dt(x)
         ga, be = _f32(gamma), _f32(beta)
-        dres = dx = dgb = None
-        if want_res:
-            dres = dout if act == 0 else torch.empty_like(x)
-        if want_dx or (want_res and act):
-            dx = torch.empty_like(x)
-        with torch.cuda.device(x.device):
-            if want_g or want_b:
-                dgb = torch.empty((2, C), device=x.device, dtype=torch.float32)
-            if dx is not None or dgb is not None:
-                chunks = _plan(l, x, S, groups, True, residual, dout)
-                part = torch.empty((N * max(chunks, 1), C, 2), device=x.device, dtype=torch.float32)
-                ab = torch.empty((N, groups, 2), device=x.device, dtype=torch.float32) if chunks else None
-                _lib.check(l.pda_group_norm_bwd(_lib.dt(x), x.data_ptr(), _lib.ptr(residual), dout.data_ptr(), _lib.ptr(dx),
-                                                _lib.ptr(dres) if act else 0, _lib.ptr(ga), _lib.ptr(be), stats.data_ptr(),
-                                                N, S, C, groups, act, cap, chunks, part.data_ptr(), _lib.ptr(ab),
-                                                0 if dgb is None else dgb[0].data_ptr(),
-                                                0 if dgb is None else dgb[1].data_ptr(), _lib.stream()),
-                           "pda_group_norm_bwd")
-        dg = dgb[0].to(gamma.dtype) if want_g else None
-        db = dgb[1].to(beta.dtype) if want_b else None
-        return dx if want_dx else None, dg, db, dres, None, None, None, None
+        with _lib.on_device_of(x):
+            chunks = _plan(l, code, N, S, C, groups, 1, x, residual, dout)
+            # one buffer: the channels' sums, (chunked) the groups' two means, the parameters' gradients
+            sums = N * (chunks or 1) * C * 2
+            means = N * groups * 2 if chunks else 0
+            work = torch.empty((sums + means,), device=x.device, dtype=torch.float32)
+            if params:
+                dg, db = (torch.empty((C,), device=x.device, dtype=torch.float32) for _ in range(2))
+            at = work.data_ptr()
+            _lib.check(l.pda_group_norm_bwd(code, x.data_ptr(), _lib.ptr(residual), dout.data_ptr(), _lib.ptr(dx),
+                                            _lib.ptr(dres) if act else 0, _lib.ptr(ga), _lib.ptr(be), stats.data_ptr(), N, S, C,
+                                            groups, act, cap, chunks, at, at + 4 * sums, _lib.ptr(dg), _lib.ptr(db),
+                                            _lib.stream()), "pda_group_norm_bwd")
+        if params:
+            dg = dg.to(gamma.dtype) if want_g else None
+            db = db.to(beta.dtype) if want_b else None
+    return dx if want_dx else None, dg, db, dres, None, None, None, None
+
+
+# under create_graph: the gradients are marked as not differentiable again
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def group_norm_act_ref(x, groups, gamma, beta, residual, act, cap, eps):
@@ -151,6 +164,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, gamma: Optional[torch.Tenso
     ``act``: ``False`` (none), ``True`` (ReLU), a positive number (ReLU clipped there, 6 for ReLU6) or ``"silu"``.
     ``gamma`` and ``beta`` (``[C]``, both or neither) keep their own dtype.  Differentiable once, in ``x``, ``gamma``,
     ``beta`` and ``residual``; a sample whose values hold a NaN or an infinity gives NaN in that group."""
+    eps = float(eps)
     groups = _check(x, num_groups, gamma, beta, residual, eps)
     code, cap = _act_code(act)
     if x.numel() == 0:
@@ -158,5 +172,5 @@ def group_norm_act(x: torch.Tensor, num_groups: int, gamma: Optional[torch.Tenso
         out = x * 1.0 if residual is None else x + residual
         return out if gamma is None else out * gamma.to(x.dtype) + beta.to(x.dtype)
     if not x.is_cuda:
-        return group_norm_act_ref(x, groups, gamma, beta, residual, code, cap, float(eps))
-    return _GroupNormActFn.apply(x, gamma, beta, residual, groups, code, cap, float(eps))
+        return group_norm_act_ref(x, groups, gamma, beta, residual, code, cap, eps)
+    return _GroupNormActFn.apply(x, gamma, beta, residual, groups, code, cap, eps)
