@@ -65,6 +65,12 @@ __device__ __forceinline__ GnVec<T, VEC> gn_ld(const T* p) { return *reinterpret
 template <typename T, int VEC>
 __device__ __forceinline__ void gn_st(T* p, const GnVec<T, VEC>& v) { *reinterpret_cast<GnVec<T, VEC>*>(p) = v; }
 
+// The channel at a place of a row, where a row may be several positions next to each other.
+__device__ __forceinline__ int gn_channel(int c, int C) {
+  while (c >= C) c -= C;
+  return c;
+}
+
 // Coefficients of the VEC channels of one thread: z = (x - mh)*sc + sh.  The mean is the fp32 pair (mh, ml), ml folded into
 // sh.  UG: the channels lie in one group, whose mean is held once.
 template <int VEC, bool UG> struct GnCoef {
@@ -77,14 +83,15 @@ template <int VEC, bool UG> struct GnCoef {
     return m;
   }
   __device__ __forceinline__ void load(const GnStat* st /* of this sample */, const float* gamma, const float* beta, int c0,
-                                       int D) {
+                                       int D, int C) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const GnStat s = st[(UG ? c0 : c0 + e) / D];
+      const int c = gn_channel(c0 + e, C);
+      const GnStat s = st[(UG ? c0 : c) / D];
       const float m = (float)s.mean;
       mh[UG ? 0 : e] = m;
-      sc[e] = (float)(s.rstd * (double)(gamma ? gamma[c0 + e] : 1.f));
-      sh[e] = (beta ? beta[c0 + e] : 0.f) - (float)(s.mean - (double)m) * sc[e];
+      sc[e] = (float)(s.rstd * (double)(gamma ? gamma[c] : 1.f));
+      sh[e] = (beta ? beta[c] : 0.f) - (float)(s.mean - (double)m) * sc[e];
     }
   }
 };
@@ -114,13 +121,14 @@ template <int ACT> __device__ __forceinline__ float gn_act(float z, float cap) {
 // Which of a vector's pre-activations lie between the borders 0 and cap, in fp64 from the fp64 statistics.
 template <typename T, int VEC>
 __device__ __forceinline__ unsigned gn_inside(const T* x, const T* res, const GnStat* st, const float* gamma, const float* beta,
-                                              int c0, int D, float cap) {
+                                              int c0, int D, int C, float cap) {
   unsigned on = 0;
 #pragma unroll 1
   for (int e = 0; e < VEC; ++e) {
-    const GnStat s = st[(c0 + e) / D];
-    const double z = ((double)ElemTraits<T>::to_f32(x[e]) - s.mean) * s.rstd * (gamma ? (double)gamma[c0 + e] : 1.0) +
-                     (beta ? (double)beta[c0 + e] : 0.0) + (res ? (double)ElemTraits<T>::to_f32(res[e]) : 0.0);
+    const int c = gn_channel(c0 + e, C);
+    const GnStat s = st[c / D];
+    const double z = ((double)ElemTraits<T>::to_f32(x[e]) - s.mean) * s.rstd * (gamma ? (double)gamma[c] : 1.0) +
+                     (beta ? (double)beta[c] : 0.0) + (res ? (double)ElemTraits<T>::to_f32(res[e]) : 0.0);
     on |= z > 0.0 && z < (double)cap ? 1u << e : 0u;
   }
   return on;
@@ -158,7 +166,7 @@ __device__ __forceinline__ float gn_silu_slope(float t, const V& w, bool wr, con
 template <int ACT, typename T, int VEC, bool UG>
 __device__ __forceinline__ void gn_grads(float (&g)[VEC], const GnVec<T, VEC>& d, const GnVec<T, VEC>& v, const GnVec<T, VEC>& w,
                                          bool wr, const GnCoef<VEC, UG>& k, const T* x, const T* res, const GnStat* st,
-                                         const float* gamma, const float* beta, int c0, int D, float cap) {
+                                         const float* gamma, const float* beta, int c0, int D, int C, float cap) {
   unsigned on = 0;
   if constexpr (gn_is_relu(ACT)) {
     GnNear near;
@@ -172,7 +180,7 @@ __device__ __forceinline__ void gn_grads(float (&g)[VEC], const GnVec<T, VEC>& d
       }
       on |= near.inside<ACT>(z, cap) ? 1u << e : 0u;
     }
-    if (near.again<ACT>(k.shmax(), cap)) on = gn_inside<T, VEC>(x, wr ? res : nullptr, st, gamma, beta, c0, D, cap);
+    if (near.again<ACT>(k.shmax(), cap)) on = gn_inside<T, VEC>(x, wr ? res : nullptr, st, gamma, beta, c0, D, C, cap);
   }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {

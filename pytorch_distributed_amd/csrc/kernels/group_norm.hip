@@ -155,7 +155,7 @@ gn_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restric
   if (g.rl >= g.RS) return;
   for (int vec = g.col; vec < vpr; vec += g.VT) {
     GnCoef<VEC, UG> k;
-    k.load(stats + (long long)n * G, gamma, beta, vec * VEC, D);
+    k.load(stats + (long long)n * G, gamma, beta, vec * VEC, D, C);
     const long long base = (long long)n * S * C + (long long)vec * VEC;
     const auto row = [&](GnVec<T, VEC>& v, const GnVec<T, VEC>& w) {
 #pragma unroll
@@ -209,12 +209,12 @@ gn_bwd_partial_kernel(const T* __restrict__ x, const T* __restrict__ res, const 
     if (active) {
       GnCoef<VEC, UG> k;
       const GnStat* stn = stats + (long long)n * G;
-      k.load(stn, gamma, beta, vec * VEC, D);
+      k.load(stn, gamma, beta, vec * VEC, D, C);
       const long long base = (long long)n * S * C + (long long)vec * VEC;
       const bool wr = ACT != GN_NONE && res;
       const auto row = [&](const GnVec<T, VEC>& v, const GnVec<T, VEC>& d, const GnVec<T, VEC>& w, long long o) {
         float gr[VEC];
-        gn_grads<ACT>(gr, d, v, w, wr, k, x + o, res + o, stn, gamma, beta, vec * VEC, D, cap);
+        gn_grads<ACT>(gr, d, v, w, wr, k, x + o, res + o, stn, gamma, beta, vec * VEC, D, C, cap);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           a[e] += gr[e];
@@ -348,7 +348,7 @@ gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, const T*
   for (int vec = g.col; vec < vpr; vec += g.VT) {
     GnCoef<VEC, UG> k;
     const GnStat* stn = stats + (long long)n * G;
-    k.load(stn, gamma, beta, vec * VEC, D);
+    k.load(stn, gamma, beta, vec * VEC, D, C);
     float pa[k.NG], pb[k.NG];
 #pragma unroll
     for (int i = 0; i < k.NG; ++i) {
@@ -360,7 +360,7 @@ gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, const T*
     const bool wr = ACT != GN_NONE && res;
     const auto row = [&](GnVec<T, VEC>& v, GnVec<T, VEC>& d, const GnVec<T, VEC>& w, long long o) {
       float gr[VEC];
-      gn_grads<ACT>(gr, d, v, w, wr, k, x + o, res + o, stn, gamma, beta, vec * VEC, D, cap);
+      gn_grads<ACT>(gr, d, v, w, wr, k, x + o, res + o, stn, gamma, beta, vec * VEC, D, C, cap);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const int i = UG ? 0 : e;
@@ -407,6 +407,12 @@ int gn_vec(int C, int esize, std::initializer_list<const void*> ptrs) {
     if (ok) return vec;
   }
   return 1;
+}
+
+bool gn_aligned(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  return true;
 }
 
 bool gn_args_ok(long long N, long long S, int C, int G, int chunks, int act) {
@@ -463,8 +469,9 @@ PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x, const void* res, voi
   if (!gn_args_ok(N, S, C, G, chunks, act)) return -1;
   const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, out});
   if (chunks == 0) {
+    const bool aligned = gn_aligned({x, res, out});
     const GnPlan p = gn_resident_plan(dtype == PDA_F32 ? 4 : 2, N, S, C, G, false);
-    if (!p.nv || vec * (dtype == PDA_F32 ? 4 : 2) != 16 || N * (C / p.W) >= (1ll << 31)) return -1;
+    if (!p.nv || !aligned || N * (C * p.fold / p.W) >= (1ll << 31)) return -1;
     const GnResidentArgs a{x, res, nullptr, out, nullptr, nullptr, gamma, beta, N, S, C, G, act, eps, cap, (GnStat*)stats,
                            nullptr, st};
     return dtype == PDA_F32 ? gn_resident_fwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_fwd<f16>(p, a)
@@ -489,8 +496,9 @@ PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x, const void* res, con
   if (!gn_args_ok(N, S, C, G, chunks, act) || (dres && !dx)) return -1;
   const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, dout, dx, dres});
   if (chunks == 0) {
+    const bool aligned = gn_aligned({x, res, dout, dx, dres});
     const GnPlan p = gn_resident_plan(dtype == PDA_F32 ? 4 : 2, N, S, C, G, true);
-    if (!p.nv || vec * (dtype == PDA_F32 ? 4 : 2) != 16 || N * (C / p.W) >= (1ll << 31)) return -1;
+    if (!p.nv || !aligned || N * (C * p.fold / p.W) >= (1ll << 31)) return -1;
     const GnResidentArgs a{x, res, dout, nullptr, dx, dres, gamma, beta, N, S, C, G, act, 0.0, act == GN_CAP ? cap : INFINITY, (GnStat*)const_cast<void*>(stats),
                            dgamma ? (float2*)part : nullptr, st};
     const int rc = dtype == PDA_F32 ? gn_resident_bwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_bwd<f16>(p, a)

@@ -12,6 +12,7 @@
 
 struct GnPlan {
   int W, threads, nv;  // nv = 0: does not fit
+  int fold = 1;        // positions that make up a row
 };
 
 // Resident vectors of one thread: what stays below the 128 registers that 1024 threads leave each.  Backward, up to
@@ -25,16 +26,21 @@ constexpr int GN_NV_FWD = 13, GN_NV_BWD = 13, GN_NV_BOTH = 7;
 inline GnPlan gn_resident_plan(int esize, long long N, long long S, int C, int G, bool bwd) {
   GnPlan best{0, 0, 0};
   const int vec = 16 / esize, D = C / G;
-  if (C % vec || S > 1024 * GN_NV_FWD) return best;
+  // channels that fill no whole vectors: as many positions a row as make them whole, and a slab is the whole row
+  int fold = 1;
+  while (C * fold % vec) fold *= 2;
+  if (S % fold || (fold > 1 && C > 4096)) return best;
+  S /= fold;
+  if (S > 1024 * GN_NV_FWD) return best;
   int a = D, b = vec;
   while (b) { const int t = a % b; a = b; b = t; }
-  const int unit = D / a * vec;  // whole groups and whole vectors
-  const int units = C / unit;
+  const int unit = fold > 1 ? C * fold : D / a * vec;  // whole groups and whole vectors
+  const int units = C * fold / unit;
   double top = 0.0;
   for (int k = 1; k <= units; ++k) {
     if (units % k) continue;
     const int W = unit * k, vt = W / vec, row = W * esize;
-    if (vt > 1024 || (row < 32 && W != C)) continue;
+    if (vt > 1024 || (row < 32 && W != C * fold)) continue;
     const long long blocks = N * (units / k);
     // both tensors in registers where 512 threads do (two workgroups on a CU), else x alone
     int threads = 0, most = bwd ? GN_NV_BOTH : GN_NV_FWD;
@@ -55,7 +61,7 @@ inline GnPlan gn_resident_plan(int esize, long long N, long long S, int C, int G
     if (bwd && nv > GN_NV_BOTH) score *= 0.9;
     if (score > top) {
       top = score;
-      best = GnPlan{W, threads, nv};
+      best = GnPlan{W, threads, nv, fold};
     }
   }
   return best;
@@ -93,8 +99,8 @@ struct GnPair { double a, b; };
 
 // Sums over every group of the slab: s[e] of every thread that is on -> s[e] of the group of slot e (UG: one slot).
 template <int VEC, bool UG>
-__device__ __forceinline__ void gn_group_totals(GnPair (&s)[UG ? 1 : VEC], double* lds, int W, int D, int RS, int col, int rl,
-                                                bool on, bool shuffles) {
+__device__ __forceinline__ void gn_group_totals(GnPair (&s)[UG ? 1 : VEC], double* lds, int W, int D, int C, int fold, int RS,
+                                                int col, int rl, bool on, bool shuffles) {
   const int VT = W / VEC, Gs = W / D, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, NW = blockDim.x >> 6;
   if constexpr (UG) {
     GnPair* buf = reinterpret_cast<GnPair*>(lds);
@@ -175,15 +181,16 @@ __device__ __forceinline__ void gn_group_totals(GnPair (&s)[UG ? 1 : VEC], doubl
 #pragma unroll
         for (int e = 0; e < VEC; ++e) lds[rl * W + col * VEC + e] = h ? s[e].b : s[e].a;
       gn_channel_totals(lds, tmp, W, RS);
-      for (int g = wave; g < Gs; g += NW) {
+      for (int g = wave; g < Gs / fold; g += NW) {
         double t = 0.0;
-        for (int d = lane; d < D; d += 64) t += lds[g * D + d];
+        for (int d = lane; d < D; d += 64)
+          for (int f = 0; f < fold; ++f) t += lds[f * C + g * D + d];
         t = wave_sum_f64(t);
         if (lane == 0) grp[g] = t;
       }
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) (h ? s[e].b : s[e].a) = grp[(col * VEC + e) / D];
+      for (int e = 0; e < VEC; ++e) (h ? s[e].b : s[e].a) = grp[(fold > 1 ? gn_channel(col * VEC + e, C) : col * VEC + e) / D];
     }
   }
 }
@@ -191,18 +198,18 @@ __device__ __forceinline__ void gn_group_totals(GnPair (&s)[UG ? 1 : VEC], doubl
 template <typename T, int NV, bool UG, int ACT>
 __global__ void __launch_bounds__(1024)
 gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ out, const float* __restrict__ gamma,
-                       const float* __restrict__ beta, int S, int C, int G, int W, double eps, float cap, int shuffles,
+                       const float* __restrict__ beta, int S, int C, int G, int W, int fold, double eps, float cap, int shuffles,
                        GnStat* __restrict__ stats) {
   extern __shared__ double lds[];
   constexpr int VEC = 16 / sizeof(T), NG = UG ? 1 : VEC;
-  const int slabs = C / W, D = C / G, VT = W / VEC, RS = blockDim.x / VT;
+  const int row = C * fold, slabs = row / W, D = C / G, VT = W / VEC, RS = blockDim.x / VT;
   const int id = xcd_remap(blockIdx.x, gridDim.x), n = id / slabs, c0 = (id % slabs) * W;
   const int col = threadIdx.x % VT, rl = threadIdx.x / VT;
   const bool on = rl < RS;
   // addresses: one for the workgroup, one offset a thread, one step a vector
-  const long long slab = (long long)n * S * C + c0;
-  unsigned off = (unsigned)(rl * C + col * VEC);
-  const auto at = [&](int i) { return slab + (long long)i * RS * C; };
+  const long long slab = (long long)n * S * row + c0;
+  unsigned off = (unsigned)(rl * row + col * VEC);
+  const auto at = [&](int i) { return slab + (long long)i * RS * row; };
   float one = 1.f;
   asm volatile("" : "+s"(one));
   GnRaw<T> v[NV];
@@ -240,8 +247,8 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
       tot[UG ? 0 : e].a += d + kp;
       tot[UG ? 0 : e].b += (double)s2[e] + p * (d + d + kp);
     }
-  gn_group_totals<VEC, UG>(tot, lds, W, D, RS, col, rl, on, shuffles);
-  const double im = 1.0 / ((double)S * D);
+  gn_group_totals<VEC, UG>(tot, lds, W, D, C, fold, RS, col, rl, on, shuffles);
+  const double im = 1.0 / ((double)S * fold * D);
   float mh[NG];
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
@@ -258,11 +265,11 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
     const double r = 1.0 / sqrt(var + eps);
     if (rl == 0) {
       const int c = c0 + col * VEC + i;  // the thread of a group's first channel writes its statistics
-      if (c % D == 0) stats[(long long)n * G + c / D] = GnStat{mean, r};
+      if (c < C && c % D == 0) stats[(long long)n * G + c / D] = GnStat{mean, r};
     }
 #pragma unroll
     for (int e = UG ? 0 : i; e < (UG ? VEC : i + 1); ++e) {
-      const int c = c0 + col * VEC + e;
+      const int c = gn_channel(c0 + col * VEC + e, C);
       sc[e] = (float)(r * (double)(gamma ? gamma[c] : 1.f));
       sh[e] = (beta ? beta[c] : 0.f) - (float)ml * sc[e];
     }
@@ -290,17 +297,17 @@ template <typename T, int NV, bool UG, int ACT>
 __global__ void __launch_bounds__(1024)
 gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout, T* __restrict__ dx,
                        T* __restrict__ dres, const float* __restrict__ gamma, const float* __restrict__ beta,
-                       const GnStat* __restrict__ stats, int S, int C, int G, int W, float cap, float2* __restrict__ part) {
+                       const GnStat* __restrict__ stats, int S, int C, int G, int W, int fold, float cap, float2* __restrict__ part) {
   extern __shared__ float2 lds2[];
   constexpr int VEC = 16 / sizeof(T);
   constexpr bool BOTH = NV <= GN_NV_BOTH;  // x and dout stay; otherwise x and (ReLUs) one bit an element of act'(z)
-  const int slabs = C / W, D = C / G, VT = W / VEC, RS = blockDim.x / VT, Gs = W / D;
+  const int row = C * fold, slabs = row / W, D = C / G, VT = W / VEC, RS = blockDim.x / VT, Gs = W / fold / D;
   const int id = xcd_remap(blockIdx.x, gridDim.x), n = id / slabs, c0 = (id % slabs) * W;
   const int col = threadIdx.x % VT, rl = threadIdx.x / VT, ct = c0 + col * VEC;
   const bool on = rl < RS;
-  const long long slab = (long long)n * S * C + c0;
-  unsigned off = (unsigned)(rl * C + col * VEC);
-  const auto at = [&](int i) { return slab + (long long)i * RS * C; };
+  const long long slab = (long long)n * S * row + c0;
+  unsigned off = (unsigned)(rl * row + col * VEC);
+  const auto at = [&](int i) { return slab + (long long)i * RS * row; };
   const auto in = [&](int i) { return on && rl + i * RS < S; };
   const bool wr = ACT != GN_NONE && res;
   const GnStat* stn = stats + (long long)n * G;
@@ -317,7 +324,7 @@ gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const
       if constexpr (BOTH) d[i] = gn_ld_raw<T>(dout + at(i) + off);
     }
   GnCoef<VEC, UG> k;
-  k.load(stn, gamma, beta, on ? ct : c0, D);
+  k.load(stn, gamma, beta, on ? ct : c0, D, C);
   float a[VEC], b[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) a[e] = b[e] = 0.f;
@@ -371,14 +378,14 @@ gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const
   if (on)
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
-      buf[rl * W + col * VEC + e] = make_float2(a[e], gn_centre(b[e], a[e], stn[(UG ? ct : ct + e) / D]));
+      buf[rl * W + col * VEC + e] = make_float2(a[e], gn_centre(b[e], a[e], stn[(UG ? ct : gn_channel(ct + e, C)) / D]));
   if constexpr (gn_is_relu(ACT))
     if (again) {  // rare: what fp64 says otherwise is put right in this thread's sums, in g and in the bits
 #pragma unroll 1
       for (int i = 0; i < NV; ++i) {
         if (!((again >> i) & 1u)) continue;
         const long long o = at(i) + off;
-        const unsigned on = gn_inside<T, VEC>(x + o, wr ? res + o : nullptr, stn, gamma, beta, ct, D, cap);
+        const unsigned on = gn_inside<T, VEC>(x + o, wr ? res + o : nullptr, stn, gamma, beta, ct, D, C, cap);
         unsigned was = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -399,7 +406,7 @@ gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const
           const float dy = ElemTraits<T>::to_f32(dout[o + e]);
           if (!(((on ^ was) >> e) & 1u) || dy == 0.f) continue;
           const float more = (on >> e) & 1u ? dy : -dy;
-          const GnStat st = stn[(ct + e) / D];
+          const GnStat st = stn[gn_channel(ct + e, C) / D];
           buf[rl * W + col * VEC + e] += make_float2(more, more * (float)(((double)ElemTraits<T>::to_f32(x[o + e]) - st.mean) * st.rstd));
         }
         if constexpr (BOTH) {
@@ -415,8 +422,13 @@ gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const
       }
     }
   gn_channel_totals(buf, tmp, W, RS);
+  if (fold > 1) {
+    for (int c = threadIdx.x; c < C; c += blockDim.x)
+      for (int f = 1; f < fold; ++f) buf[c] += buf[f * C + c];
+    __syncthreads();
+  }
   if (part)
-    for (int c = threadIdx.x; c < W; c += blockDim.x) part[(long long)n * C + c0 + c] = buf[c];
+    for (int c = threadIdx.x; c < W / fold; c += blockDim.x) part[(long long)n * C + c0 + c] = buf[c];
   if (!dx) return;
   for (int g = threadIdx.x >> 6; g < Gs; g += blockDim.x >> 6) {
     double ta = 0.0, tb = 0.0;
@@ -429,7 +441,7 @@ gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const
     ta = wave_sum_f64(ta);
     tb = wave_sum_f64(tb);
     if ((threadIdx.x & 63) == 0) {
-      const double m = (double)S * D;
+      const double m = (double)S * fold * D;
       grp[g] = make_float2((float)(ta / m), (float)(tb / m));
     }
   }
@@ -438,7 +450,7 @@ gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const
   float pa[k.NG], pb[k.NG];
 #pragma unroll
   for (int i = 0; i < k.NG; ++i) {
-    const int g = (col * VEC + i) / D;
+    const int g = (fold > 1 ? gn_channel(col * VEC + i, C) : col * VEC + i) / D;
     gn_dx_coefs(grp[g].x, grp[g].y, stn[c0 / D + g], pa[i], pb[i]);
   }
   gn_renew(off);
@@ -503,11 +515,11 @@ template <typename K> static int gn_allow_lds(K kernel, size_t lds) {
 template <typename T, int NV, bool UG, int ACT> static int gn_launch_fwd(const GnPlan& p, const GnResidentArgs& a) {
   constexpr int VEC = 16 / sizeof(T);
   const int D = a.C / a.G, vt = p.W / VEC, dv = D / VEC;
-  const int shuffles = vt <= 64 && (vt & (vt - 1)) == 0 && (UG ? (dv & (dv - 1)) == 0 : VEC % D == 0);
+  const int shuffles = p.fold == 1 && vt <= 64 && (vt & (vt - 1)) == 0 && (UG ? (dv & (dv - 1)) == 0 : VEC % D == 0);
   const size_t lds = gn_fwd_lds(p.W, p.threads, VEC, D);
   if (int rc = gn_allow_lds(gn_resident_fwd_kernel<T, NV, UG, ACT>, lds)) return rc;
-  hipLaunchKernelGGL((gn_resident_fwd_kernel<T, NV, UG, ACT>), dim3((unsigned)(a.N * (a.C / p.W))), dim3(p.threads), lds, a.st,
-                     (const T*)a.x, (const T*)a.res, (T*)a.out, a.gamma, a.beta, (int)a.S, a.C, a.G, p.W, a.eps, a.cap, shuffles,
+  hipLaunchKernelGGL((gn_resident_fwd_kernel<T, NV, UG, ACT>), dim3((unsigned)(a.N * (a.C * p.fold / p.W))), dim3(p.threads), lds,
+                     a.st, (const T*)a.x, (const T*)a.res, (T*)a.out, a.gamma, a.beta, (int)(a.S / p.fold), a.C, a.G, p.W, p.fold, a.eps, a.cap, shuffles,
                      a.stats);
   return pda_check_launch();
 }
@@ -515,9 +527,9 @@ template <typename T, int NV, bool UG, int ACT> static int gn_launch_bwd(const G
   constexpr int VEC = 16 / sizeof(T);
   const size_t lds = gn_bwd_lds(p.W, p.threads, VEC, a.C / a.G);
   if (int rc = gn_allow_lds(gn_resident_bwd_kernel<T, NV, UG, ACT>, lds)) return rc;
-  hipLaunchKernelGGL((gn_resident_bwd_kernel<T, NV, UG, ACT>), dim3((unsigned)(a.N * (a.C / p.W))), dim3(p.threads), lds, a.st,
-                     (const T*)a.x, (const T*)a.res, (const T*)a.dout, (T*)a.dx, (T*)a.dres, a.gamma, a.beta, a.stats, (int)a.S,
-                     a.C, a.G, p.W, a.cap, a.part);
+  hipLaunchKernelGGL((gn_resident_bwd_kernel<T, NV, UG, ACT>), dim3((unsigned)(a.N * (a.C * p.fold / p.W))), dim3(p.threads), lds,
+                     a.st, (const T*)a.x, (const T*)a.res, (const T*)a.dout, (T*)a.dx, (T*)a.dres, a.gamma, a.beta, a.stats,
+                     (int)(a.S / p.fold), a.C, a.G, p.W, p.fold, a.cap, a.part);
   return pda_check_launch();
 }
 #define GN_RES_ACT(FN, NV, UG)                                                      \

@@ -110,6 +110,11 @@ SHAPES = [  # shape, groups
     ((257, 2, 2, 512), 32),     # many small samples
     ((3, 40), 5),               # no positions at all
     ((2, 50, 24), 4),
+    ((3, 6, 6, 58), 2),         # several positions make up whole vectors
+    ((2, 4, 4, 7), 7),
+    ((2, 8, 3, 12), 3),
+    ((1, 120, 120, 24), 3),     # too many positions for registers
+    ((9, 28, 28, 64), 32),
 ]
 
 
