@@ -54,6 +54,15 @@ def build_parser(description: str = "PyTorch ImageNet Training", arch: str = "re
     p.add_argument("--opt-level", default=None, choices=["O0", "O1", "O2", "O3"])
     p.add_argument("--bucket-mb", default=25.0, type=float)
     p.add_argument("--sync-bn", action="store_true")
+    p.add_argument("--group-norm", default=0, type=int, metavar="G",
+                   help="group norm of G groups in place of every BatchNorm (0 = keep BatchNorm)")
+    p.add_argument("--teacher", default="", metavar="ARCH", choices=[""] + models.model_names,
+                   help="distil from this architecture: its top logits are scored beside the labels")
+    p.add_argument("--teacher-checkpoint", default="", type=str, metavar="PATH", help="weights of the teacher")
+    p.add_argument("--distill-top", default=32, type=int, metavar="K", help="teacher logits kept per image")
+    p.add_argument("--distill-temperature", default=4.0, type=float, metavar="T")
+    p.add_argument("--distill-weight", default=0.5, type=float, metavar="W",
+                   help="loss = (1 - W) * cross-entropy + W * distillation")
     p.add_argument("--resume", default="", type=str, metavar="PATH")
     p.add_argument("--steps-per-epoch", default=0, type=int, help="cap iterations per epoch (0 = full)")
     p.add_argument("--jsonl", default="", type=str, help="per-step JSONL log (rank 0)")
@@ -85,7 +94,45 @@ def make_model(args, device):
     if args.sync_bn:
         from .nn import SyncBatchNorm
         SyncBatchNorm.convert_sync_batchnorm(model)
+    if getattr(args, "group_norm", 0):
+        from .nn import GroupNorm
+        GroupNorm.convert_group_norm(model, args.group_norm)
     return model.to(device)
+
+
+class Teacher:
+    """A frozen model whose top logits a student is trained on beside the labels (``--teacher``)."""
+
+    def __init__(self, model, k: int = 32, temperature: float = 4.0, weight: float = 0.5):
+        if not 0.0 <= weight <= 1.0:
+            raise ValueError(f"the weight of the distillation loss must lie between 0 and 1, not {weight}")
+        self.model = model.eval()
+        for p in self.model.parameters():
+            p.requires_grad_(False)
+        self.k, self.temperature, self.weight = int(k), float(temperature), float(weight)
+
+    def loss(self, images: torch.Tensor, output: torch.Tensor, label_loss: torch.Tensor) -> torch.Tensor:
+        """``(1 - weight) * label_loss + weight * distillation`` of the student's ``output`` on ``images``."""
+        with torch.no_grad():
+            values, indices, rest = ops.top_logits(self.model(images), min(self.k, output.shape[-1]), self.temperature)
+        soft = ops.distill_loss(output, values, indices, rest, self.temperature)
+        return (1.0 - self.weight) * label_loss + self.weight * soft
+
+
+def make_teacher(args, device) -> Optional[Teacher]:
+    """The teacher that ``--teacher`` asks for, or None.  It reads the same batches as the student, with the same head."""
+    if not getattr(args, "teacher", ""):
+        return None
+    model = models.get_model(args.teacher, num_classes=args.num_classes) if args.teacher != "mnist_net" else models.Net()
+    if args.teacher_checkpoint:
+        utils.load_checkpoint(args.teacher_checkpoint, model)
+    dtype = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}[args.precision]
+    if hasattr(model, "set_compute_dtype") and torch.device(device).type == "cuda":
+        model.set_compute_dtype(dtype)
+    norm = getattr(args, "input_uint8", None)
+    if norm is not None and hasattr(model, "set_input_normalization"):
+        model.set_input_normalization(norm[0], norm[1], 1.0 / 255.0)
+    return Teacher(model.to(device), args.distill_top, args.distill_temperature, args.distill_weight)
 
 
 def make_optimizer(args, model, fused: bool = True):
@@ -111,7 +158,7 @@ def _rank():
 
 
 def train(loader, model, criterion, optimizer, epoch: int, device, args, zero_grad: Optional[Callable] = None,
-          scale_loss: bool = True, jsonl: Optional[utils.JsonlLogger] = None):
+          scale_loss: bool = True, jsonl: Optional[utils.JsonlLogger] = None, teacher: Optional[Teacher] = None):
     batch_time = utils.AverageMeter("Time", ":6.3f")
     data_time = utils.AverageMeter("Data", ":6.3f")
     losses = utils.AverageMeter("Loss", ":.4e")
@@ -143,6 +190,8 @@ def train(loader, model, criterion, optimizer, epoch: int, device, args, zero_gr
             loss = criterion(output, target, metrics.buf) if _takes_metrics(criterion) else criterion(output, target)
             if not _takes_metrics(criterion):
                 ops.loss.update_metrics_ref(output.detach().float(), target, metrics.buf)
+            if teacher is not None:
+                loss = teacher.loss(images, output, loss)
         (zero_grad or optimizer.zero_grad)()
         with utils.annotate("backward"):
             if scale_loss and getattr(optimizer, "_amp_scaler_ref", None) is not None:
@@ -301,6 +350,10 @@ def fit(args, model, optimizer, device, train_set, val_set, per_rank_batch: int,
             print(f"=> resumed from '{args.resume}' (epoch {args.start_epoch})")
     if args.evaluate:
         return validate(val_loader, model, criterion, device, args, val_sampler)
+    teacher = make_teacher(args, device)
+    if teacher is not None and norm is not None and (prefetch_norm is None) != hasattr(teacher.model,
+                                                                                        "set_input_normalization"):
+        raise ValueError("--teacher: teacher and student take raw image bytes in different ways; choose architectures of one kind")
     csv = utils.EpochCSV(csv_path) if (csv_path and chief) else None
     jsonl = utils.JsonlLogger(args.jsonl) if args.jsonl else None
     # failure detection for the whole run: a rank that dies (or a link that goes away under a collective) ends
@@ -312,14 +365,14 @@ def fit(args, model, optimizer, device, train_set, val_set, per_rank_batch: int,
     try:
         best_acc1 = _fit_epochs(args, model, optimizer, device, criterion, train_loader, val_loader, train_sampler,
                                 val_sampler, prefetch_norm, pin, zero_grad, csv, jsonl, chief, best_acc1,
-                                save_prefix_arch)
+                                save_prefix_arch, teacher)
     finally:
         stop_watchdog()
     return best_acc1
 
 
 def _fit_epochs(args, model, optimizer, device, criterion, train_loader, val_loader, train_sampler, val_sampler,
-                prefetch_norm, pin, zero_grad, csv, jsonl, chief, best_acc1, save_prefix_arch):
+                prefetch_norm, pin, zero_grad, csv, jsonl, chief, best_acc1, save_prefix_arch, teacher=None):
     for epoch in range(args.start_epoch, args.epochs):
         t0 = time.time()
         if train_sampler is not None:
@@ -328,7 +381,7 @@ def _fit_epochs(args, model, optimizer, device, criterion, train_loader, val_loa
         utils.adjust_learning_rate(optimizer, epoch, args.lr)
         tl = DevicePrefetcher(train_loader, device, normalize=prefetch_norm, channels_scale=255.0) \
             if (pin or prefetch_norm is not None) else train_loader
-        train(tl, model, criterion, optimizer, epoch, device, args, zero_grad, jsonl=jsonl)
+        train(tl, model, criterion, optimizer, epoch, device, args, zero_grad, jsonl=jsonl, teacher=teacher)
         acc1 = validate(val_loader, model, criterion, device, args, val_sampler)
         is_best = acc1 > best_acc1
         best_acc1 = max(acc1, best_acc1)

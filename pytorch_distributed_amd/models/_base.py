@@ -34,7 +34,7 @@ class NHWCModel(tnn.Module):
 
 def run_layers(layers, x: torch.Tensor) -> torch.Tensor:
     """``nn.Sequential`` semantics with one peephole: ``Conv2d, BatchNorm2d[, ReLU]`` runs as the fused
-    conv + BatchNorm (+ ReLU) op, ``BatchNorm2d, ReLU`` as one normalise-and-activate pass and
+    conv + BatchNorm (+ ReLU) op, ``BatchNorm2d, ReLU`` / ``GroupNorm, ReLU`` as one normalise-and-activate pass and
     ``Conv2d, ReLU`` with the activation inside the conv's bias pass."""
     mods = list(layers)
     i, n = 0, len(mods)
@@ -45,7 +45,7 @@ def run_layers(layers, x: torch.Tensor) -> torch.Tensor:
             relu = i + 2 < n and isinstance(mods[i + 2], pnn.ReLU)
             x = pnn.ConvBnAct.run(m, nxt, x, relu=relu)
             i += 3 if relu else 2
-        elif isinstance(m, pnn.BatchNorm2d) and isinstance(nxt, pnn.ReLU):
+        elif isinstance(m, (pnn.BatchNorm2d, pnn.GroupNorm)) and isinstance(nxt, pnn.ReLU):
             x = m(x, None, True)
             i += 2
         elif isinstance(m, pnn.Conv2d) and isinstance(nxt, pnn.ReLU) and not m._forward_hooks:

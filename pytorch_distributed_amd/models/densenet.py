@@ -94,7 +94,7 @@ class DenseNet(NHWCModel):
 
     def forward(self, images: torch.Tensor) -> torch.Tensor:
         f = self.features
-        if f.conv0.out_channels == 64:
+        if f.conv0.out_channels == 64 and isinstance(f.norm0, pnn.BatchNorm2d):
             # same stem as the ResNets: layout change, conv, BatchNorm, ReLU and pool as one fused op
             x = ops.stem_conv_bn_relu_pool(images, f.conv0.weight, f.norm0.weight, f.norm0.bias, f.conv0.stride,
                                            f.conv0.padding, f.norm0.state(), self.compute_dtype,

@@ -249,11 +249,22 @@ class ResNet(tnn.Module):
         self.compute_dtype = dtype
         return self
 
+    def _stem(self, images: torch.Tensor) -> torch.Tensor:
+        if not isinstance(self.bn1, pnn.BatchNorm2d):   # group norm: the layers one by one
+            x = images
+            if self._in_mean is not None or self.input_scale != 1.0:
+                x = x.float() * self.input_scale
+            if self._in_mean is not None:
+                x = (x - self._in_mean.view(1, -1, 1, 1)) * self._in_inv_std.view(1, -1, 1, 1)
+            x = pnn.to_nhwc(x.to(self.compute_dtype))
+            return self.maxpool(self.bn1(self.conv1(x), None, True))
+        return ops.stem_conv_bn_relu_pool(images, self.conv1.weight, self.bn1.weight, self.bn1.bias, self.conv1.stride,
+                                          self.conv1.padding, self.bn1.state(), self.compute_dtype,
+                                          pool=(self.maxpool.kernel_size, self.maxpool.stride, self.maxpool.padding),
+                                          mean=self._in_mean, inv_std=self._in_inv_std, pre_scale=self.input_scale)
+
     def features(self, images: torch.Tensor) -> torch.Tensor:
-        x = ops.stem_conv_bn_relu_pool(images, self.conv1.weight, self.bn1.weight, self.bn1.bias, self.conv1.stride,
-                                       self.conv1.padding, self.bn1.state(), self.compute_dtype,
-                                       pool=(self.maxpool.kernel_size, self.maxpool.stride, self.maxpool.padding),
-                                       mean=self._in_mean, inv_std=self._in_inv_std, pre_scale=self.input_scale)
+        x = self._stem(images)
         # block by block (what nn.Sequential would do) so that each block's backward link reaches the
         # block that consumes its output; the link is dropped from the modules right away - only the
         # autograd nodes of this forward keep it

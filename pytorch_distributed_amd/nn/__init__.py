@@ -10,7 +10,7 @@ num_batches_tracked``.  Activations flowing between these modules are physically
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 import torch.nn as tnn
@@ -107,6 +107,51 @@ class SyncBatchNorm(BatchNorm2d):
         return module
 
 
+class GroupNorm(tnn.Module):
+    """Group norm over the channel (last) dimension of an ``[N, ..., C]`` tensor: statistics of one sample's
+    ``num_channels / num_groups`` adjacent channels, the same in training and evaluation, nothing crosses ranks."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True):
+        super().__init__()
+        if num_groups <= 0 or num_channels % num_groups:
+            raise ValueError("num_channels must be divisible by num_groups")
+        self.num_groups, self.num_channels, self.eps, self.affine = num_groups, num_channels, eps, affine
+        if affine:
+            self.weight = tnn.Parameter(torch.ones(num_channels))
+            self.bias = tnn.Parameter(torch.zeros(num_channels))
+        else:
+            self.register_parameter("weight", None)
+            self.register_parameter("bias", None)
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                act: Union[bool, float, str] = False) -> torch.Tensor:
+        """``act``: ``False``, ``True`` (ReLU), a positive number (ReLU clipped there) or ``"silu"``."""
+        return ops.group_norm_act(x, self.num_groups, self.weight, self.bias, residual, act, self.eps)
+
+    def extra_repr(self) -> str:
+        return f"{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.affine}, layout=NHWC"
+
+    @classmethod
+    def convert_group_norm(cls, module: tnn.Module, num_groups: int) -> tnn.Module:
+        """Replace every BatchNorm2d of this package inside ``module`` (in place; weights and biases are taken over, running
+        statistics go) by group norm of ``num_groups`` groups, or of the greatest common divisor where the channels do not
+        divide by it.  To be called before the optimizer and a distributed wrapper take the parameters."""
+        if num_groups <= 0:
+            raise ValueError("num_groups must be positive")
+        for parent in list(module.modules()):
+            for name, m in list(parent.named_children()):
+                if not isinstance(m, BatchNorm2d):
+                    continue
+                g = cls(math.gcd(num_groups, m.num_features), m.num_features, m.eps, m.affine)
+                if m.affine:
+                    g.weight, g.bias = m.weight, m.bias
+                g.train(m.training)
+                setattr(parent, name, g)
+            if hasattr(parent, "fuse_relu_backward"):
+                parent.fuse_relu_backward(False)   # those hand-offs ride on the convs' BatchNorm epilogues
+        return module
+
+
 class _ZeroGradFor(torch.autograd.Function):
     """Identity on ``out`` that also hands ``param`` an all-zero gradient (so that optimizers and gradient
     reducers see every parameter of the step)."""
@@ -142,7 +187,7 @@ class ConvBnAct(tnn.Module):
         """``mask_dx`` / ``dout_premasked`` / ``in_link`` / ``out_link`` / ``res_in`` / ``res_out`` / ``alias_link``: see
         :func:`pytorch_distributed_amd.ops.conv_bn_act`."""
         pointwise = conv.kernel_size == (1, 1) and conv.stride == (1, 1) and conv.padding == (0, 0)
-        fused_path = (conv.bias is None and conv.groups == 1 and conv.out_channels % 8 == 0
+        fused_path = (isinstance(bn, BatchNorm2d) and conv.bias is None and conv.groups == 1 and conv.out_channels % 8 == 0
                       and bool(_conv.igemm_tiles(conv.in_channels, x.dtype))
                       and (pointwise or bool(_conv.igemm_tiles(conv.out_channels, x.dtype))))
         if res_in is not None and res_in.affine is not None and not fused_path:
@@ -150,7 +195,7 @@ class ConvBnAct(tnn.Module):
             from ..ops.fused import materialize_shortcut
             residual, res_in = materialize_shortcut(residual, res_in), None
         plain = not (passthrough or mask_dx or dout_premasked or in_link is not None or out_link is not None)
-        if (conv.bias is not None and plain and x.is_cuda and bn.training and bn.track_running_stats
+        if (isinstance(bn, BatchNorm2d) and conv.bias is not None and plain and x.is_cuda and bn.training and bn.track_running_stats
                 and bn.momentum is not None and conv.groups == 1 and conv.out_channels % 8 == 0
                 and _conv.igemm_tiles(conv.in_channels, x.dtype)
                 and (pointwise or _conv.igemm_tiles(conv.out_channels, x.dtype))):
@@ -162,10 +207,10 @@ class ConvBnAct(tnn.Module):
             with torch.no_grad():
                 bn.running_mean.add_(conv.bias.detach().to(bn.running_mean.dtype), alpha=bn.momentum)
             return _ZeroGradFor.apply(o, conv.bias)
-        if conv.bias is not None or conv.groups != 1 or conv.out_channels % 8 \
+        if not isinstance(bn, BatchNorm2d) or conv.bias is not None or conv.groups != 1 or conv.out_channels % 8 \
                 or not _conv.igemm_tiles(conv.in_channels, x.dtype) \
                 or not (pointwise or _conv.igemm_tiles(conv.out_channels, x.dtype)):
-            # unfused modules (a bias, groups, or a channel count the MFMA kernels do not tile): the BatchNorm op masks its own ReLU gradient (dout_premasked needs nothing, a
+            # unfused modules (group norm, a bias, groups, or a channel count the MFMA kernels do not tile): the BatchNorm op masks its own ReLU gradient (dout_premasked needs nothing, a
             # link given to it stays empty), and the promise made by mask_dx / in_link is kept by an explicit
             # gradient mask on x
             if in_link is not None and in_link.mat is not None:
@@ -279,6 +324,20 @@ class CrossEntropyLoss(tnn.Module):
         return ops.cross_entropy(logits, target, metrics, self.reduction)
 
 
+class DistillationLoss(tnn.Module):
+    """Distillation from a teacher's top logits (``ops.distill_loss``; ``ops.top_logits`` makes the entries)."""
+
+    def __init__(self, temperature: float = 1.0, reduction: str = "mean"):
+        super().__init__()
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, logits, top_values, top_indices, rest: Optional[torch.Tensor] = None):
+        return ops.distill_loss(logits, top_values, top_indices, rest, self.temperature, self.reduction)
+
+    def extra_repr(self) -> str:
+        return f"temperature={self.temperature}, reduction={self.reduction!r}"
+
+
 def to_nhwc(x: torch.Tensor) -> torch.Tensor:
     """NCHW -> physically NHWC tensor of shape [N,H,W,C]."""
     return x.permute(0, 2, 3, 1).contiguous()
@@ -288,6 +347,6 @@ def to_nchw(x: torch.Tensor) -> torch.Tensor:
     return x.permute(0, 3, 1, 2).contiguous()
 
 
-__all__ = ["Conv2d", "BatchNorm2d", "SyncBatchNorm", "ConvBnAct", "ReLU", "ReLU6", "MaxPool2d", "AvgPool2d",
+__all__ = ["Conv2d", "BatchNorm2d", "SyncBatchNorm", "GroupNorm", "DistillationLoss", "ConvBnAct", "ReLU", "ReLU6", "MaxPool2d", "AvgPool2d",
            "AdaptiveAvgPool2d", "GlobalAvgPool2d", "Dropout",
            "Dropout2d", "Linear", "CrossEntropyLoss", "to_nhwc", "to_nchw"]

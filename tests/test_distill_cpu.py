@@ -44,6 +44,7 @@ def test_distill_loss_is_the_divergence_of_all_classes(t):
     v, i, r = ops.top_logits(teacher, 9, t)
     want = F.kl_div(F.log_softmax(z.double() / t, 1), F.softmax(teacher.double() / t, 1), reduction="none").sum(1) * t * t
     gw, = torch.autograd.grad(want.mean(), z)
+    want = want.detach()
     for rest in (None, r):
         loss = ops.distill_loss(z, v, i, rest, t)
         assert abs(float(loss.detach()) - float(want.mean())) < 1e-6
@@ -132,3 +133,51 @@ def test_distill_loss_no_rows_and_leading_dimensions():
     assert torch.equal(loss.reshape(-1), flat)
     e = ops.distill_loss(torch.empty(0, 9), torch.empty(0, 4), torch.empty(0, 4, dtype=torch.int64), None, 1.0, "sum")
     assert float(e) == 0.0
+
+
+def test_distillation_module_and_teacher():
+    from pytorch_distributed_amd import engine
+    torch.manual_seed(0)
+    teacher_model, student = models.Net(), models.Net()
+    teacher = engine.Teacher(teacher_model, k=4, temperature=2.0, weight=0.25)
+    assert not teacher.model.training and not any(p.requires_grad for p in teacher.model.parameters())
+    x = torch.randn(3, 1, 28, 28)
+    student.eval()
+    out = student(x)
+    label = F.cross_entropy(out.float(), torch.tensor([1, 2, 3]))
+    loss = teacher.loss(x, out, label)
+    with torch.no_grad():
+        v, i, r = ops.top_logits(teacher_model(x), 4, 2.0)
+    want = 0.75 * label + 0.25 * pnn.DistillationLoss(2.0)(out, v, i, r)
+    assert abs(float(loss.detach()) - float(want.detach())) < 1e-6
+    loss.backward()
+    assert all(p.grad is None for p in teacher_model.parameters()) and any(bool(p.grad.any()) for p in student.parameters())
+    with pytest.raises(ValueError):
+        engine.Teacher(teacher_model, weight=1.5)
+
+
+def test_group_norm_student_of_a_teacher_trains():
+    """The operators together: a group norm student's gradients through the distillation loss, against differences."""
+    torch.manual_seed(3)
+    conv = pnn.Conv2d(3, 16, 3, 1, 1)
+    gn = pnn.GroupNorm(4, 16)
+    fc = pnn.Linear(16, 12)
+    x, teacher_logits = torch.randn(2, 6, 6, 3), torch.randn(2, 12) * 3
+    v, i, r = ops.top_logits(teacher_logits, 5, 2.0)
+
+    def loss():
+        return ops.distill_loss(fc(gn(conv(x), None, "silu").mean((1, 2))), v, i, r, 2.0)
+
+    params = [gn.weight, gn.bias, fc.weight]
+    grads = torch.autograd.grad(loss(), params)
+    h = 2.0 ** -6
+    for p, g in zip(params, grads):
+        for k in (0, p.numel() - 1):
+            with torch.no_grad():
+                p.view(-1)[k] += h
+                hi = float(loss())
+                p.view(-1)[k] -= 2 * h
+                lo = float(loss())
+                p.view(-1)[k] += h
+            # h^2 times a third derivative below 4, and the rounding of fp32 losses below 4
+            assert abs((hi - lo) / (2 * h) - float(g.reshape(-1)[k])) < 4 * h * h + 2.0 ** -24 * 4 * 16 / h

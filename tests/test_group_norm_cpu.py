@@ -68,3 +68,65 @@ def test_group_norm_act_refusals():
         ops.group_norm_act(x.double(), 4)
     with pytest.raises(ValueError):
         ops.group_norm_act(torch.randn(8), 4)
+
+
+def test_group_norm_module_and_refusals():
+    from pytorch_distributed_amd import nn as pnn
+    m = pnn.GroupNorm(4, 8)
+    x = torch.randn(2, 3, 3, 8)
+    assert torch.equal(m(x, x, True), ops.group_norm_act(x, 4, m.weight, m.bias, x, True))
+    assert pnn.GroupNorm(2, 8, affine=False)(x).shape == x.shape
+    for a in [(3, 8), (0, 8)]:
+        with pytest.raises(ValueError):
+            pnn.GroupNorm(*a)
+
+
+@pytest.mark.parametrize("arch", ["resnet18", "resnext50_32x4d", "vgg11_bn", "densenet121", "mobilenet_v2", "shufflenet_v2_x0_5",
+                                  "mnasnet0_5", "googlenet"])
+def test_group_norm_in_place_of_batch_norm(arch):
+    """Every family runs with group norm: one sample's logits do not depend on its batch, nor on training mode."""
+    from pytorch_distributed_amd import nn as pnn, models
+    torch.manual_seed(0)
+    m = models.get_model(arch, num_classes=7)
+    names = [n for n, _ in m.named_parameters()]
+    pnn.GroupNorm.convert_group_norm(m, 32)
+    assert [n for n, _ in m.named_parameters()] == names
+    assert not any(isinstance(k, pnn.BatchNorm2d) for k in m.modules())
+    for k in m.modules():
+        if isinstance(k, pnn.Dropout):
+            k.p = 0.0
+    x = torch.randn(2, 3, 64, 64)
+    m.train()
+    out = m(x)
+    # fp32 through some fifty layers, summed in another order for another batch size
+    torch.testing.assert_close(m(x[:1]), out[:1], rtol=1e-3, atol=1e-3 * float(out.detach().abs().max()))
+    out.square().mean().backward()
+    grads = [p.grad for k in m.modules() if isinstance(k, pnn.GroupNorm) for p in (k.weight, k.bias)]
+    assert all(g is not None and bool(torch.isfinite(g).all()) for g in grads)
+    assert any(bool(g.any()) for g in grads)
+
+
+def test_group_norm_resnet_layers_one_by_one():
+    """The converted ResNet against the same parameters in torch.nn.functional, values and gradients."""
+    from pytorch_distributed_amd import nn as pnn, models
+    torch.manual_seed(1)
+    m = pnn.GroupNorm.convert_group_norm(models.resnet18(num_classes=5), 16)
+    m.set_input_normalization([0.4, 0.5, 0.6], [0.2, 0.3, 0.25], 0.5)
+    x = torch.rand(2, 3, 40, 40)
+
+    def gn(k, t):
+        return F.group_norm(t, k.num_groups, k.weight, k.bias, k.eps)
+
+    y = (x * 0.5 - torch.tensor([0.4, 0.5, 0.6]).view(1, 3, 1, 1)) / torch.tensor([0.2, 0.3, 0.25]).view(1, 3, 1, 1)
+    y = F.max_pool2d(torch.relu(gn(m.bn1, F.conv2d(y, m.conv1.weight, None, 2, 3))), 3, 2, 1)
+    for b in [b for l in (m.layer1, m.layer2, m.layer3, m.layer4) for b in l]:
+        r = y if b.downsample is None else gn(b.downsample[1], F.conv2d(y, b.downsample[0].weight, None, b.stride))
+        t = torch.relu(gn(b.bn1, F.conv2d(y, b.conv1.weight, None, b.stride, 1)))
+        y = torch.relu(gn(b.bn2, F.conv2d(t, b.conv2.weight, None, 1, 1)) + r)
+    want = m.fc(y.mean((2, 3)))
+    gw = torch.autograd.grad(want.sum(), [m.conv1.weight, m.layer3[0].bn2.weight])
+    got = m(x)
+    gg = torch.autograd.grad(got.sum(), [m.conv1.weight, m.layer3[0].bn2.weight])
+    torch.testing.assert_close(got, want, rtol=1e-3, atol=1e-4)
+    for a, b in zip(gg, gw):
+        torch.testing.assert_close(a, b, rtol=1e-2, atol=1e-3 * float(b.abs().max()))

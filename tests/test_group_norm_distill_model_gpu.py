@@ -1,0 +1,59 @@
+"""Group norm students of a teacher on the GPU: the converted models against the same parameters on the CPU, and a whole
+step of both operators recorded and replayed."""
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from pytorch_distributed_amd import engine, models, nn as pnn, ops, utils
+
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("arch,groups", [("resnet18", 32), ("densenet121", 16), ("shufflenet_v2_x1_0", 8), ("mobilenet_v2", 8)])
+def test_converted_model_matches_the_cpu(arch, groups):
+    """fp32 on both sides: the bound is that of fp32 convolutions through the depth of the networks."""
+    torch.manual_seed(0)
+    cpu = pnn.GroupNorm.convert_group_norm(models.get_model(arch, num_classes=9), groups)
+    for m in cpu.modules():
+        if isinstance(m, pnn.Dropout):
+            m.p = 0.0
+    gpu = copy.deepcopy(cpu).to(DEV)
+    x, t = torch.randn(4, 3, 64, 64), torch.randint(0, 9, (4,))
+    out, ref = gpu(x.to(DEV)), cpu(x)
+    torch.testing.assert_close(out.cpu(), ref, rtol=2e-3, atol=2e-3 * float(ref.detach().abs().max()))
+    v, i, r = ops.top_logits(torch.randn(4, 9) * 2, 4, 2.0)
+    (ops.cross_entropy(ref, t) + ops.distill_loss(ref, v, i, r, 2.0)).backward()
+    (ops.cross_entropy(out, t.to(DEV)) + ops.distill_loss(out, v.to(DEV), i.to(DEV), r.to(DEV), 2.0)).backward()
+    for (n, a), (_, b) in zip(gpu.named_parameters(), cpu.named_parameters()):
+        err = float((a.grad.cpu() - b.grad).norm() / (b.grad.norm() + 1e-6))
+        assert err < 2e-2, (n, err)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_student_and_teacher_step_recorded(dtype):
+    torch.manual_seed(1)
+    student = pnn.GroupNorm.convert_group_norm(models.resnet18(num_classes=40), 32).set_compute_dtype(dtype).to(DEV)
+    teacher = engine.Teacher(models.resnet18(num_classes=40).set_compute_dtype(dtype).to(DEV), k=8, temperature=2.0, weight=0.5)
+    x, t = torch.randn(8, 3, 64, 64, device=DEV), torch.randint(0, 40, (8,), device=DEV)
+    params = list(student.parameters())
+
+    def step():
+        out = student(x)
+        loss = teacher.loss(x, out, ops.cross_entropy(out, t))
+        return (loss.detach(),) + torch.autograd.grad(loss, params)
+
+    step()
+    graphed = utils.GraphedStep(step, warmup=2)
+    assert graphed.captured
+    for k in range(3):
+        x.copy_(torch.randn(8, 3, 64, 64, device=DEV))
+        got = [g.clone() for g in graphed()]
+        torch.cuda.synchronize()
+        want = step()
+        assert abs(float(got[0]) - float(want[0])) <= 1e-3 * (1 + abs(float(want[0])))
+        for p, a, b in zip(params, got[1:], want[1:]):
+            # weight gradients of the convolutions are summed in an order that varies
+            assert float((a - b).norm()) <= 2e-2 * float(b.norm()) + 1e-5, p.shape
