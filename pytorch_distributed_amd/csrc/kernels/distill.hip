@@ -1,8 +1,9 @@
 // Distillation from a teacher's top logits: the selection of a row's k largest logits (with the log-sum-exp of the others)
 // and the Kullback-Leibler loss of a student against them, forward and backward.
 //
-// Rows have one stride, their elements are adjacent; a row starts anywhere (odd class counts), so the 16-byte accesses
-// are typed as element-aligned.  One block takes one row; sums of a row's terms are fp32 over a few hundred elements a
+// Rows have one stride, their elements are adjacent; a row starts anywhere (odd class counts).  The 16-byte accesses are
+// typed as element-aligned; where a row is written, its first elements are taken alone up to the next 16 bytes.  (Where one is
+// summed up they are not: that costs 5 % on rows of 50001 16-bit classes, but sums do not depend on where a tensor lies.)  One block takes one row; sums of a row's terms are fp32 over a few hundred elements a
 // thread, what the loss is made of (k entries and three log-sum-exps a row) is fp64: student and teacher are nearly equal
 // late in training and their logarithms cancel.
 #include "common.h"
@@ -26,6 +27,12 @@ __device__ __forceinline__ RowVec<T> row_ld(const T* p) {
 }
 template <typename T>
 __device__ __forceinline__ void row_st(T* p, const RowVec<T>& r) { __builtin_memcpy(p, &r, 16); }
+
+// Elements in front of the first one on a 16-byte address.
+template <typename T> __device__ __forceinline__ int row_head(const T* p, int V) {
+  const int h = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T);
+  return h < V ? h : V;
+}
 
 // Running maximum (raw logit) and sum of exp((z - m)/T).  m starts at the lowest finite number, so that neither a row of
 // infinities nor a difference of two of them makes a NaN that the row has not got.
@@ -583,34 +590,35 @@ distill_bwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
   const float gr = g[rowi * gstride] * gscale;
   const RowStat st = stat[rowi];
   const float f = st.factor * gr;
-  const int nv = V / VN;
+  const int head = row_head(out, V), nv = (V - head) / VN;
+  const auto end = [&](int o) { return o < head ? o : nv * VN + o; };  // the o-th of the elements outside the vectors
   if (st.factor == 0.f) {  // not read: what stands in a row without entries may be anything
     RowVec<T> v;
 #pragma unroll
     for (int e = 0; e < VN; ++e) v.v[e] = ElemTraits<T>::from_f32(0.f);
-    for (int i = threadIdx.x; i < nv; i += NT) row_st(out + (long long)i * VN, v);
-    for (int j = nv * VN + threadIdx.x; j < V; j += NT) out[j] = ElemTraits<T>::from_f32(0.f);
+    for (int i = threadIdx.x; i < nv; i += NT) row_st(out + head + (long long)i * VN, v);
+    for (int o = threadIdx.x; o < V - nv * VN; o += NT) out[end(o)] = ElemTraits<T>::from_f32(0.f);
   } else {
     const auto value = [&](float zf) { return fast_exp2<T>((zf - st.shift) * c) * f; };
     const auto put = [&](RowVec<T>& v, int i) {
 #pragma unroll
       for (int e = 0; e < VN; ++e) v.v[e] = ElemTraits<T>::from_f32(value(ElemTraits<T>::to_f32(v.v[e])));
-      row_st(out + (long long)i * VN, v);
+      row_st(out + head + (long long)i * VN, v);
     };
     constexpr int U = 4;
     int i = threadIdx.x;
     for (; i + (U - 1) * NT < nv; i += U * NT) {
       RowVec<T> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = row_ld(row + (long long)(i + u * NT) * VN);
+      for (int u = 0; u < U; ++u) v[u] = row_ld(row + head + (long long)(i + u * NT) * VN);
 #pragma unroll
       for (int u = 0; u < U; ++u) put(v[u], i + u * NT);
     }
     for (; i < nv; i += NT) {
-      RowVec<T> v = row_ld(row + (long long)i * VN);
+      RowVec<T> v = row_ld(row + head + (long long)i * VN);
       put(v, i);
     }
-    for (int j = nv * VN + threadIdx.x; j < V; j += NT) out[j] = ElemTraits<T>::from_f32(value(ElemTraits<T>::to_f32(row[j])));
+    for (int o = threadIdx.x; o < V - nv * VN; o += NT) out[end(o)] = ElemTraits<T>::from_f32(value(ElemTraits<T>::to_f32(row[end(o)])));
   }
   __syncthreads();
   for (int k = threadIdx.x; k < K; k += NT) {
