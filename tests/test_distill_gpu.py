@@ -187,6 +187,13 @@ def test_distill_loss_sizes(rows, V, k, t, dtype):
     check_loss(z, v, i, r, t)
 
 
+def test_distill_loss_gradient_larger_than_the_caches():
+    z = logits(270, 131071, torch.bfloat16, 20)
+    v, i, r = teacher(z, 8, 2.0, 21)
+    i[::7] = -1
+    check_loss(z, v, i, r, 2.0)
+
+
 @pytest.mark.parametrize("with_rest", [False, True])
 def test_distill_loss_masks(with_rest):
     rows, V, k, t = 12, 513, 6, 2.0
