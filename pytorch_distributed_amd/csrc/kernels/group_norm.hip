@@ -1,10 +1,9 @@
 // Group norm with an optional residual and activation, channels last: x [N][S][C], C = G groups of D channels.  The formulas
 // are those of group_norm.h.
 //
-// Statistics: a thread takes its rows in batches of four, relative to the first row of its chunk (a mean far from zero
-// costs no digits), forms each batch's mean and centred squares in fp32 and adds batches up in fp64; (sample, group)
-// totals are fp64 and kept as pairs {mu, r}.  16-bit inputs lose next to nothing in a batch, so their statistics are good
-// to far below fp32; a value next to an activation's border is placed by them in fp64.
+// Statistics are sums of x and x^2 in fp64 (the products are exact there, and a mean far from zero may be taken off
+// afterwards) and are kept in fp64: a value next to an activation's border is placed by them.  The element passes take mu as
+// an fp32 pair (hi subtracted from x, lo folded into the shift).
 //
 // Memory-bound throughout: the work is split over (sample, row chunk), a thread owns one vector of channels and walks
 // rows, so the per-channel coefficients stay in registers.  No atomics: results repeat bit for bit.
@@ -26,26 +25,10 @@ struct GnGeom {
   }
 };
 
-// Sums of one channel over some rows, relative to a pivot: a = sum (x - pivot), b = sum (x - pivot)^2.
+// Sum of x and of x^2.
 struct GnSums { double a, b; };
 
-// Four values of a channel (or one) added to its sums.  b takes the squares around the batch's own mean and that mean's
-// square in fp64, so a pivot far out (an outlier in the first row) costs no digits of the spread.
-__device__ __forceinline__ void gn_add4(GnSums& s, const float (&f)[4]) {
-  const float mb = ((f[0] + f[1]) + (f[2] + f[3])) * 0.25f;
-  float q = 0.f;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) { const float d = f[u] - mb; q += d * d; }
-  const double m4 = (double)mb * 4.0;
-  s.a += m4;
-  s.b += (double)q + m4 * (double)mb;
-}
-__device__ __forceinline__ void gn_add1(GnSums& s, float f) {
-  s.a += (double)f;
-  s.b += (double)f * (double)f;
-}
-
-// Per-channel sums of one row chunk (pivot: its first row) -> part[n][chunk][c].
+// Per-channel sums of one row chunk -> part[n][chunk][c].
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 gn_partial_kernel(const T* __restrict__ x, long long S, int C, int chunks, GnSums* __restrict__ part) {
@@ -63,25 +46,23 @@ gn_partial_kernel(const T* __restrict__ x, long long S, int C, int chunks, GnSum
     for (int e = 0; e < VEC; ++e) s[e] = GnSums{0.0, 0.0};
     if (active) {
       const T* p = xn + (long long)vec * VEC;
-      const GnVec<T, VEC> pivot = gn_ld<T, VEC>(p + r0 * C);
+      const auto add = [&](const GnVec<T, VEC>& v) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const double f = (double)v.f(e);
+          s[e].a += f;
+          s[e].b += f * f;
+        }
+      };
       long long r = r0 + g.rl;
       for (; r + 3 * g.RS < r1; r += 4 * g.RS) {
         GnVec<T, VEC> v[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) v[u] = gn_ld<T, VEC>(p + (r + u * g.RS) * C);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float p0 = ElemTraits<T>::to_f32(pivot.v[e]);
-          const float f[4] = {ElemTraits<T>::to_f32(v[0].v[e]) - p0, ElemTraits<T>::to_f32(v[1].v[e]) - p0,
-                              ElemTraits<T>::to_f32(v[2].v[e]) - p0, ElemTraits<T>::to_f32(v[3].v[e]) - p0};
-          gn_add4(s[e], f);
-        }
+        for (int u = 0; u < 4; ++u) add(v[u]);
       }
-      for (; r < r1; r += g.RS) {
-        const GnVec<T, VEC> v = gn_ld<T, VEC>(p + r * C);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) gn_add1(s[e], ElemTraits<T>::to_f32(v.v[e]) - ElemTraits<T>::to_f32(pivot.v[e]));
-      }
+      for (; r < r1; r += g.RS) add(gn_ld<T, VEC>(p + r * C));
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sm[e * 256 + threadIdx.x] = s[e];
@@ -109,37 +90,24 @@ gn_partial_kernel(const T* __restrict__ x, long long S, int C, int chunks, GnSum
 }
 
 // One wave per (sample, group): chunks x D sums -> {mu, r} in fp64.
-template <typename T>
 __global__ void __launch_bounds__(64)
-gn_finalize_kernel(const T* __restrict__ x, const GnSums* __restrict__ part, long long S, int C, int G, int chunks, double eps,
+gn_finalize_kernel(const GnSums* __restrict__ part, long long S, int C, int G, int chunks, double eps,
                    GnStat* __restrict__ stats) {
   const int D = C / G;
   const int n = blockIdx.x / G, g = blockIdx.x % G;
   const GnSums* p = part + (long long)n * chunks * C + (long long)g * D;
-  const T* xg = x + (long long)n * S * C + (long long)g * D;
   const long long pairs = (long long)chunks * D;
-  double a = 0.0;
+  double a = 0.0, b = 0.0;
   for (long long j = threadIdx.x; j < pairs; j += 64) {
-    const int ch = (int)(j / D), d = (int)(j % D);
-    const long long r0 = S * ch / chunks;
-    const double k = (double)(S * (ch + 1) / chunks - r0);
-    a += k * (double)ElemTraits<T>::to_f32(xg[r0 * C + d]) + p[(long long)ch * C + d].a;
+    const GnSums v = p[(j / D) * C + j % D];
+    a += v.a;
+    b += v.b;
   }
   const double m = (double)S * D;
   const double mean = wave_sum_f64(a) / m;
-  double q = 0.0;
-  for (long long j = threadIdx.x; j < pairs; j += 64) {
-    const int ch = (int)(j / D), d = (int)(j % D);
-    const long long r0 = S * ch / chunks;
-    const double k = (double)(S * (ch + 1) / chunks - r0);
-    const GnSums v = p[(long long)ch * C + d];
-    const double own = v.a / k;                       // this channel's mean over the chunk, from the pivot
-    const double e = (double)ElemTraits<T>::to_f32(xg[r0 * C + d]) + own - mean;
-    const double c = v.b - v.a * own;                 // squares around it
-    q += (c > 0.0 ? c : c != c ? c : 0.0) + k * e * e;
-  }
-  q = wave_sum_f64(q);
-  if (threadIdx.x == 0) stats[blockIdx.x] = GnStat{mean, 1.0 / sqrt(q / m + eps)};
+  double var = wave_sum_f64(b) / m - mean * mean;
+  var = var < 0.0 ? 0.0 : var;  // (a NaN stays one)
+  if (threadIdx.x == 0) stats[blockIdx.x] = GnStat{mean, 1.0 / sqrt(var + eps)};
 }
 
 template <typename T, int VEC, bool UG, int ACT>
@@ -480,8 +448,8 @@ PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x, const void* res, voi
   const int blocks = (int)(N * chunks);
   GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x, S, C,
                                              chunks, (GnSums*)part));
-  GN_DISPATCH(dtype, 1, hipLaunchKernelGGL((gn_finalize_kernel<E>), dim3((int)(N * G)), dim3(64), 0, st, (const E*)x,
-                                           (const GnSums*)part, S, C, G, chunks, eps, (GnStat*)stats));
+  hipLaunchKernelGGL(gn_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const GnSums*)part, S, C, G, chunks, eps,
+                     (GnStat*)stats);
   const bool ug = (C / G) % vec == 0;
   GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_apply_kernel<E, VEC, UG, ACT>), dim3(blocks), dim3(256),
               0, st, (const E*)x, (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, cap)));

@@ -20,6 +20,17 @@ struct GnPlan {
 // caches).
 constexpr int GN_NV_FWD = 13, GN_NV_BWD = 13, GN_NV_BOTH = 7;
 
+// Shared memory of a workgroup: the larger of what the ways of gn_group_totals use; gn_channel_totals with its input.
+inline size_t gn_fwd_lds(int W, int threads, int vec, int D) {
+  const size_t waves = 16ull * (threads / 64) * (W / D);  // a pair for each wave and group
+  const size_t all = D % vec == 0 ? 16ull * (threads + W / D)
+                                  : 8ull * ((size_t)(threads / (W / vec)) * W + (threads > W ? threads : W) + W / D);
+  return waves > all ? waves : all;
+}
+inline size_t gn_bwd_lds(int W, int threads, int vec, int D) {
+  return 8ull * ((size_t)(threads / (W / vec)) * W + (threads > W ? threads : W) + W / D);
+}
+
 // Measured on 400 samples, fp16, forward / backward: the width of a slab's rows counts most (56x56x256 with residual:
 // 16 bytes 701 / 1381 us, 32 bytes 530 / 973, 64 bytes 443 us forward), up to 128 bytes (14x14x1024: 32 bytes 114 / 202, 64 bytes
 // 101 / 183, 128 bytes 108 / 194), then few threads with many vectors (28x28x512: 512 threads 197, 1024 230 us).
@@ -50,6 +61,7 @@ inline GnPlan gn_resident_plan(int esize, long long N, long long S, int C, int G
       most = bwd ? GN_NV_BWD : GN_NV_FWD;
     }
     if (!threads) continue;
+    if ((bwd ? gn_bwd_lds(W, 1024, vec, D) : gn_fwd_lds(W, 1024, vec, D)) > 156 * 1024) continue;
     // few blocks: more threads each, while their vectors stay two or more
     while (threads < 1024 && blocks * threads < 256 * 512 && (S + threads / vt - 1) / (threads / vt) > 3) threads *= 2;
     const int nv = (int)((S + threads / vt - 1) / (threads / vt));
@@ -85,14 +97,6 @@ template <typename V> __device__ __forceinline__ void gn_channel_totals(V* buf, 
     buf[c] = a;
   }
   __syncthreads();
-}
-
-inline size_t gn_fwd_lds(int W, int threads, int vec, int D) {
-  if (D % vec == 0) return 16ull * (threads + (size_t)(threads / 64 + 1) * (W / D));
-  return 8ull * ((size_t)(threads / (W / vec)) * W + (threads > W ? threads : W) + 2 * (W / D));
-}
-inline size_t gn_bwd_lds(int W, int threads, int vec, int D) {
-  return 8ull * ((size_t)(threads / (W / vec)) * W + (threads > W ? threads : W) + W / D);
 }
 
 struct GnPair { double a, b; };
@@ -217,36 +221,21 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (in(i)) v[i] = gn_ld_raw<T>(x + at(i) + off);
-  // A thread's rows relative to its first one, in fp32 (an outlier there raises the variance with its own rounding); from
-  // there in fp64, where the square of a mean may be taken off the mean of the squares.
-  float s1[VEC], s2[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) s1[e] = s2[e] = 0.f;
-  float p0[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) p0[e] = v[0].f(e);
-  int cnt = in(0) ? 1 : 0;
-#pragma unroll
-  for (int i = 1; i < NV; ++i)
-    if (in(i)) {
-      ++cnt;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d = v[i].sub(e, p0[e], one);
-        s1[e] += d;
-        s2[e] += d * d;
-      }
-    }
+  // Sums of x and of x^2 in fp64: the products are exact there, a mean far from zero may be taken off afterwards, and the side
+  // of an activation's border on which an element lies can be decided by what comes out (a sum of squares in fp32, joined
+  // in fp64, put one element of 300 million on the wrong one).
   GnPair tot[NG];
 #pragma unroll
   for (int i = 0; i < NG; ++i) tot[i] = GnPair{0.0, 0.0};
-  if (cnt)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const double p = (double)p0[e], kp = (double)cnt * p, d = (double)s1[e];
-      tot[UG ? 0 : e].a += d + kp;
-      tot[UG ? 0 : e].b += (double)s2[e] + p * (d + d + kp);
-    }
+  for (int i = 0; i < NV; ++i)
+    if (in(i))
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const double f = (double)v[i].f(e);
+        tot[UG ? 0 : e].a += f;
+        tot[UG ? 0 : e].b += f * f;
+      }
   gn_group_totals<VEC, UG>(tot, lds, W, D, C, fold, RS, col, rl, on, shuffles);
   const double im = 1.0 / ((double)S * fold * D);
   float mh[NG];

@@ -114,7 +114,10 @@ class Teacher:
     def loss(self, images: torch.Tensor, output: torch.Tensor, label_loss: torch.Tensor) -> torch.Tensor:
         """``(1 - weight) * label_loss + weight * distillation`` of the student's ``output`` on ``images``."""
         with torch.no_grad():
-            values, indices, rest = ops.top_logits(self.model(images), min(self.k, output.shape[-1]), self.temperature)
+            logits = self.model(images)
+            if logits.shape != output.shape:
+                raise ValueError(f"the teacher's logits are {tuple(logits.shape)}, the student's {tuple(output.shape)}")
+            values, indices, rest = ops.top_logits(logits, min(self.k, logits.shape[-1]), self.temperature)
         soft = ops.distill_loss(output, values, indices, rest, self.temperature)
         return (1.0 - self.weight) * label_loss + self.weight * soft
 

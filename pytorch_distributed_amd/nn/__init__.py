@@ -138,15 +138,19 @@ class GroupNorm(tnn.Module):
         divide by it.  To be called before the optimizer and a distributed wrapper take the parameters."""
         if num_groups <= 0:
             raise ValueError("num_groups must be positive")
+
+        def converted(m: BatchNorm2d) -> "GroupNorm":
+            g = cls(math.gcd(num_groups, m.num_features), m.num_features, m.eps, m.affine)
+            if m.affine:
+                g.weight, g.bias = m.weight, m.bias
+            return g.train(m.training)
+
+        if isinstance(module, BatchNorm2d):
+            return converted(module)
         for parent in list(module.modules()):
             for name, m in list(parent.named_children()):
-                if not isinstance(m, BatchNorm2d):
-                    continue
-                g = cls(math.gcd(num_groups, m.num_features), m.num_features, m.eps, m.affine)
-                if m.affine:
-                    g.weight, g.bias = m.weight, m.bias
-                g.train(m.training)
-                setattr(parent, name, g)
+                if isinstance(m, BatchNorm2d):
+                    setattr(parent, name, converted(m))
             if hasattr(parent, "fuse_relu_backward"):
                 parent.fuse_relu_backward(False)   # those hand-offs ride on the convs' BatchNorm epilogues
         return module

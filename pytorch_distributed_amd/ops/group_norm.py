@@ -6,6 +6,7 @@ this is the normalisation that needs neither running statistics nor SyncBatchNor
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Union
 
 import torch
@@ -62,13 +63,21 @@ def _f32(p):
     return p.detach().float().contiguous()
 
 
-def _plan(l, code: int, N: int, S: int, C: int, groups: int, backward: int, *tensors) -> int:
-    """0: a sample's groups stay in registers; otherwise the row chunks of the multi-pass kernels."""
-    aligned = all(t is None or t.data_ptr() % 16 == 0 for t in tensors)
-    chunks = l.pda_group_norm_plan(code, N, S, C, groups, backward, int(aligned))
+@functools.lru_cache(maxsize=4096)
+def _plan_of(code: int, N: int, S: int, C: int, groups: int, backward: int, aligned: bool) -> int:
+    chunks = _lib.lib().pda_group_norm_plan(code, N, S, C, groups, backward, int(aligned))
     if chunks < 0:
         _lib.check(chunks, "pda_group_norm_plan")
     return chunks
+
+
+def _plan(code: int, N: int, S: int, C: int, groups: int, backward: int, *tensors) -> int:
+    """0: a sample's groups stay in registers; otherwise the row chunks of the multi-pass kernels."""
+    aligned = True
+    for t in tensors:
+        if t is not None and t.data_ptr() % 16:
+            aligned = False
+    return _plan_of(code, N, S, C, groups, backward, aligned)
 
 
 class _GroupNormActFn(torch.autograd.Function):
@@ -84,7 +93,7 @@ class _GroupNormActFn(torch.autograd.Function):
         out = torch.empty_like(x)
         ga, be = _f32(gamma), _f32(beta)
         with _lib.on_device_of(x):
-            chunks = _plan(l, code, N, S, C, groups, 0, x, residual)
+            chunks = _plan(code, N, S, C, groups, 0, x, residual)
             part = torch.empty((N * chunks, C, 2), device=x.device, dtype=torch.float64) if chunks else None
             stats = torch.empty((N, groups, 2), device=x.device, dtype=torch.float64)
             _lib.check(l.pda_group_norm_fwd(code, x.data_ptr(), _lib.ptr(residual), out.data_ptr(), _lib.ptr(ga), _lib.ptr(be),
@@ -116,7 +125,7 @@ def _backward(ctx, dout):
         code = _lib.dt(x)
         ga, be = _f32(gamma), _f32(beta)
         with _lib.on_device_of(x):
-            chunks = _plan(l, code, N, S, C, groups, 1, x, residual, dout)
+            chunks = _plan(code, N, S, C, groups, 1, x, residual, dout)
             # one buffer: the channels' sums, (chunked) the groups' two means, the parameters' gradients
             sums = N * (chunks or 1) * C * 2
             means = N * groups * 2 if chunks else 0

@@ -263,6 +263,27 @@ def test_distill_loss_strides():
     check_loss(z[:1].expand(10, 901), v[:1].expand(10, 8), i[:1].expand(10, 8), r[:1].expand(10), 2.0)
 
 
+def test_distill_loss_one_row_and_differentiable_once():
+    z = logits(1, 333, torch.float32, 22)[0].requires_grad_(True)
+    v, i, r = teacher(z.detach(), 7, 2.0, 23)
+    for rest in (None, r):
+        a = ops.distill_loss(z, v, i, rest, 2.0, "none")
+        assert a.shape == () and torch.equal(a, ops.distill_loss(z[None], v[None], i[None], None if rest is None else rest[None],
+                                                                 2.0, "none")[0])
+        assert torch.autograd.grad(a, z)[0].shape == (333,)
+    loss = ops.distill_loss(z, v, i, r, 2.0)
+    g, = torch.autograd.grad(loss, z, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    loss = ops.distill_loss(z, v, i, r, 2.0)
+    with torch.no_grad():
+        z += 1.0
+    with pytest.raises(RuntimeError):    # changed in place since the forward pass
+        torch.autograd.grad(loss, z)
+    values, indices, rest = ops.top_logits(z, 5)
+    assert not values.requires_grad and not rest.requires_grad
+
+
 def test_distill_loss_no_rows():
     z = torch.empty((0, 9), device=DEV, requires_grad=True)
     loss = ops.distill_loss(z, torch.empty((0, 4), device=DEV), torch.empty((0, 4), device=DEV, dtype=torch.int64), None, 1.0, "sum")

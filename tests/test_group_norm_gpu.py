@@ -115,6 +115,10 @@ SHAPES = [  # shape, groups
     ((2, 8, 3, 12), 3),
     ((1, 120, 120, 24), 3),     # too many positions for registers
     ((9, 28, 28, 64), 32),
+    ((40, 2, 2, 512), 512),     # a group a channel, rows as wide as a wave
+    ((1500, 1, 3, 512), 512),
+    ((1100, 1, 2, 4096), 4096),
+    ((3, 2, 3, 2048), 128),
 ]
 
 
@@ -158,6 +162,25 @@ def test_group_norm_act_borders_of_the_activation():
     out = ops.group_norm_act(x, 2, w, b, rl, True)
     dres = torch.autograd.grad(out, rl, dy)[0]
     assert torch.equal((dres != 0)[sure], (left > 0)[sure] & (dy != 0)[sure])
+
+
+@pytest.mark.parametrize("shape,groups", [((2, 300, 8), 2), ((3, 28, 28, 64), 8), ((2, 56, 56, 32), 16), ((2, 15000, 8), 2),
+                                          ((2, 9, 11, 58), 29)])
+@pytest.mark.parametrize("act", [True, 6.0])
+def test_group_norm_act_side_of_a_border_is_that_of_fp64(shape, groups, act):
+    """As above with values of full precision: sums of x and x^2 in fp64 are off by 1e-16 times the root of their number at
+    most (300 here), z by a few of those; 1e-12 is beyond it."""
+    x, w, b, _, dy = make(shape, torch.float32, 31)
+    z = exact(x, groups, w, b, None, False, 1e-5)["out"][0].reshape(shape)
+    border = 0.0 if act is True else 6.0
+    res = (border - z).float()
+    left = z + res.double() - border
+    sure = left.abs() > 1e-12
+    assert float(sure.double().mean()) > 0.9
+    rl = res.requires_grad_(True)
+    dres, = torch.autograd.grad(ops.group_norm_act(x, groups, w, b, rl, act), rl, dy)
+    inside = left > 0 if act is True else left < 0
+    assert torch.equal((dres != 0)[sure], inside[sure] & (dy != 0)[sure])
 
 
 def test_group_norm_act_constant_groups_and_nan():
@@ -204,6 +227,21 @@ def test_group_norm_act_gradient_subsets_and_parameter_types():
     # no activation: the residual's gradient is the upstream one
     r2 = res.clone().requires_grad_(True)
     assert torch.equal(torch.autograd.grad(ops.group_norm_act(x, 4, None, None, r2), r2, dy)[0], dy)
+
+
+def test_group_norm_act_is_differentiable_once():
+    x, w, b, _, dy = make((2, 3, 3, 16), torch.float32, 15)
+    xl = x.requires_grad_(True)
+    out = ops.group_norm_act(xl, 4, w, b, None, "silu")
+    g, = torch.autograd.grad(out, xl, dy, create_graph=True)
+    close("dx", g.detach(), exact(x, 4, w, b, None, "silu", 1e-5, dy)["dx"])
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    out = ops.group_norm_act(xl, 4, w, b, None, True)
+    with torch.no_grad():
+        xl += 1.0
+    with pytest.raises(RuntimeError):    # changed in place since the forward pass
+        torch.autograd.grad(out, xl, dy)
 
 
 def test_group_norm_act_same_tensor_twice_and_retained_graph():
