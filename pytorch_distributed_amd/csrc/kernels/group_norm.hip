@@ -6,7 +6,9 @@
 // an fp32 pair (hi subtracted from x, lo folded into the shift).
 //
 // Memory-bound throughout: the work is split over (sample, row chunk), a thread owns one vector of channels and walks
-// rows, so the per-channel coefficients stay in registers.  No atomics: results repeat bit for bit.
+// rows, so the per-channel coefficients stay in registers; 2048 blocks of two or four rows in flight a thread measured
+// best (128x112x112x64 bf16 with SiLU: sums 49 us = 4.2 TB/s, apply 77 us = 5.3, backward sums 117 us, bound by the sigmoid,
+// backward apply 120 us = 5.1).  No atomics: results repeat bit for bit.
 #include "group_norm_resident.h"
 
 #include <initializer_list>
