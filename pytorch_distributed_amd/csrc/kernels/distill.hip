@@ -58,28 +58,30 @@ template <typename T> __device__ __forceinline__ float fast_exp2(float x) {
   return sizeof(T) == 4 ? exp2f(x) : __builtin_amdgcn_exp2f(x);
 }
 // The same running pair for whole vectors, on the scale that the exponential takes: sum of 2^(z*c - mc) with one
-// multiply-add an element.  mc is the rounded product of the maximum and c; flush() takes its rounding out of the sum.
-// A sum of 0 can also mean that every value is the lowest fp32 number: the caller looks again with ms_add then.
+// multiply-add an element.  mc is the rounded product of the maximum and c; flush() takes its rounding out of the sum.  Where
+// the product is so large that its rounding matters by itself (masks of the type's lowest value, tiny temperatures), and
+// where a NaN or +inf came by, the sum is given as NaN: the caller then looks again with ms_add, which takes differences first.
 struct FastSum {
-  float m = -FLT_MAX, mc = 0.f, s = 0.f;
-  __device__ __forceinline__ void raise(float m2, float c) {
-    const float mc2 = m2 * c;
-    s *= s == 0.f ? 0.f : __builtin_amdgcn_exp2f(mc - mc2);
-    m = m2;
-    mc = mc2;
-  }
+  float m = -INFINITY, mc = 0.f, s = 0.f;
   template <int N> __device__ __forceinline__ void add(const float (&z)[N], float c) {
     float top = z[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, z[e]);
-    if (top > m) raise(top, c);
+    if (top > m) {
+      const float mc2 = top * c;
+      s *= s == 0.f ? 0.f : __builtin_amdgcn_exp2f(mc - mc2);
+      m = top;
+      mc = mc2;
+    }
     float a = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) a += __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], c, -mc));
     s += a;
   }
   __device__ __forceinline__ MaxSum flush(float c) const {
-    return MaxSum{m, s == 0.f ? 0.f : s * __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -mc))};
+    if (m == -INFINITY) return MaxSum{-FLT_MAX, s};  // nothing, or infinities below (or NaN alone: s is one)
+    if (!(fabsf(mc) <= 16777216.f)) return MaxSum{m, NAN};
+    return MaxSum{m, s * __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -mc))};
   }
 };
 template <int NT>
@@ -482,16 +484,13 @@ distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
   }
   for (; i < nv; i += NT) take(fetch(i), i);
   MaxSum ms = fs.flush(c);
+  const bool odd = !(ms.s < INFINITY);
   const auto skipped = [&](int j) { return rest && ((en.bits[j >> 5] >> (j & 31)) & 1u); };
-  for (int j = nv * VN + threadIdx.x; j < V; j += NT)
+  const int from = __syncthreads_or(odd) ? 0 : nv * VN;  // the last elements, or all of them again
+  if (from == 0) ms = MaxSum{-FLT_MAX, 0.f};
+  for (int j = from + threadIdx.x; j < V; j += NT)
     if (!skipped(j)) ms_add(ms, ElemTraits<T>::to_f32(row[j]), c);
   ms = ms_block<NT>(ms, c, scratch);
-  if (ms.s == 0.f) {  // nothing above the lowest number
-    ms = MaxSum{-FLT_MAX, 0.f};
-    for (int j = threadIdx.x; j < V; j += NT)
-      if (!skipped(j)) ms_add(ms, ElemTraits<T>::to_f32(row[j]), c);
-    ms = ms_block<NT>(ms, c, scratch);
-  }
   if (twice)  // rare: entries of one class are one class of the distribution
     for (int k = threadIdx.x; k < K; k += NT)
       if (en.idx[k] >= 0)
@@ -500,22 +499,24 @@ distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
   __syncthreads();
   if (threadIdx.x >= 64) return;
   const int lane = threadIdx.x;
-  // student: L = log sum exp(z/T) over everything, lt over the remainder (with rest)
-  // (a softmax that holds +inf is NaN, as everywhere else)
-  const double lt = ms.m == INFINITY ? (double)NAN : (double)ms.m * it + log((double)ms.s);
-  double L = lt;
+  // Student: log q of an entry is (z - M)/T - lS with the maximum M of everything and S = sum exp((z - M)/T); all logarithms
+  // are taken next to a maximum, where masks of -1e38 do not swallow them.  (A softmax that holds +inf is NaN, as
+  // everywhere else.)
+  const double m = (double)ms.m, ls = log((double)ms.s);
+  double M = m, S = ms.m == INFINITY ? (double)NAN : (double)ms.s;
   if (rest) {
-    double m = -DBL_MAX;
+    double me = -DBL_MAX;
     for (int k = lane; k < K; k += 64)
-      if (en.idx[k] >= 0) m = max_nan(m, (double)en.z[k] * it);
-    m = wave_max_d(m);
-    double s = 0.0;
+      if (en.idx[k] >= 0) me = max_nan(me, (double)en.z[k]);
+    me = wave_max_d(me);
+    double se = 0.0;
     for (int k = lane; k < K; k += 64)
-      if (en.idx[k] >= 0 && en.first[k] == k) s += exp((double)en.z[k] * it - m);
-    s = wave_sum_d(s);
-    const double le = m + log(s), hi = max_nan(le, lt);
-    L = hi + log(exp(le - hi) + exp(lt - hi));
+      if (en.idx[k] >= 0 && en.first[k] == k) se += exp(((double)en.z[k] - me) * it);
+    se = wave_sum_d(se);
+    M = max_nan(m, me);
+    S = S * exp((m - M) * it) + (se == 0.0 ? 0.0 : se * exp((me - M) * it));
   }
+  const double lS = log(S);
   // teacher
   const double R = rest ? (double)rest[rowi] : -INFINITY;
   double tm = -INFINITY;
@@ -540,32 +541,32 @@ distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
     if (en.idx[k] >= 0) ts += exp(en.p[k] - tm);
   ts = wave_sum_d(ts);
   if (rest) ts += exp(R - tm);
-  const double lz = tm + log(ts);
+  const double lts = log(ts);
   double loss = 0.0;
   for (int k = lane; k < K; k += 64) {
     const int j = en.idx[k];
     double d = 0.0;
     if (j >= 0) {
-      double lp = en.p[k] - lz, p = exp(lp);
+      double lp = (en.p[k] - tm) - lts, p = exp(lp);
       if (twice) {
         p = 0.0;
         for (int o = 0; o < K; ++o)
-          if (en.idx[o] == j) p += exp(en.p[o] - lz);
+          if (en.idx[o] == j) p += exp((en.p[o] - tm) - lts);
         lp = log(p);
       }
-      const double lq = (double)en.z[k] * it - L;
+      const double lq = ((double)en.z[k] - M) * it - lS;
       if (en.first[k] == k && p != 0.0) loss += p * (lp - lq);
       d = exp(lq) - p;
     }
     dtop[rowi * K + k] = (float)d;
   }
   loss = wave_sum_d(loss);
-  // q of the remainder against its own maximum: q_j = exp((z_j - m)/T) * alpha
-  double factor = exp((double)ms.m * it - L);
+  // q of the remainder against its own maximum: q_j = exp((z_j - m)/T) * factor
+  double factor = exp((m - M) * it - lS);
   if (rest) {
-    const double pr = exp(R - lz);
+    const double pr = exp((R - tm) - lts);
     if (pr != 0.0) {
-      loss += pr * ((R - lz) - (lt - L));
+      loss += pr * (((R - tm) - lts) - ((m - M) * it + ls - lS));
       factor -= pr / (double)ms.s;
     }
     if (ms.s == 0.f) factor = 0.0;

@@ -420,7 +420,7 @@ bool gn_args_ok(long long N, long long S, int C, int G, int chunks, int act) {
 // How a call runs: 0 = a slab of a sample in registers (group_norm_resident.h), > 0 = that many row chunks a sample, in
 // passes.  aligned: every tensor starts on 16 bytes.
 PDA_EXPORT int pda_group_norm_plan(int dtype, long long N, long long S, int C, int G, int bwd, int aligned) {
-  if (N <= 0 || S <= 0 || C <= 0 || G <= 0 || C % G) return -1;
+  if (N <= 0 || S <= 0 || C <= 0 || C > (1 << 28) || G <= 0 || C % G) return -1;
   const int es = dtype == PDA_F32 ? 4 : 2;
   if (aligned && gn_resident_plan(es, N, S, C, G, bwd != 0).nv) return 0;
   // about 2048 blocks over the chip, at least 8 rows for each thread of a block

@@ -37,10 +37,11 @@ inline size_t gn_bwd_lds(int W, int threads, int vec, int D) {
 inline GnPlan gn_resident_plan(int esize, long long N, long long S, int C, int G, bool bwd) {
   GnPlan best{0, 0, 0};
   const int vec = 16 / esize, D = C / G;
+  if (C > (1 << 20)) return best;  // offsets in a workgroup are 32 bits
   // channels that fill no whole vectors: as many positions a row as make them whole, and a slab is the whole row
   int fold = 1;
   while (C * fold % vec) fold *= 2;
-  if (S % fold || (fold > 1 && C > 4096) || C > (1 << 20)) return best;  // (offsets in a workgroup are 32 bits)
+  if (S % fold || (fold > 1 && C > 4096)) return best;
   S /= fold;
   if (S > 1024 * GN_NV_FWD) return best;
   int a = D, b = vec;

@@ -8,6 +8,7 @@ the kernels of ``csrc/kernels/distill.hip``; CPU path = stock PyTorch math.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -16,14 +17,15 @@ from . import _lib
 
 MAX_K = 1024
 MAX_CLASSES = 1 << 20
+MIN_TEMPERATURE, MAX_TEMPERATURE = 2.0 ** -20, 2.0 ** 20
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _temperature(t) -> float:
     t = float(t)
-    if not (0.0 < t < math.inf):
-        raise ValueError(f"temperature must be a positive number, not {t}")
+    if not (MIN_TEMPERATURE <= t <= MAX_TEMPERATURE):
+        raise ValueError(f"temperature must lie between {MIN_TEMPERATURE} and {MAX_TEMPERATURE}, not {t}")
     return t
 
 
@@ -62,10 +64,11 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> Tuple[
 
     ``values`` ``[..., k]`` descend and keep the logits' dtype; of equal ones the lowest class comes first, and NaN counts
     as larger than every number.  ``indices`` are int64.  ``rest`` (fp32, ``[...]``) is
-    ``log(sum(exp(z_j / temperature)))`` over the classes that were not taken, -inf where there are none.  Not
-    differentiable.  ``1 <= k <= min(classes, 1024)``."""
+    ``log(sum(exp(z_j / temperature)))`` over the classes that were not taken, -inf where there are none (and an
+    infinity where it leaves fp32: logits near fp32's ends with a temperature below one).  Not differentiable.
+    ``1 <= k <= min(classes, 1024)``, ``2^-20 <= temperature <= 2^20``."""
     _check_logits("top_logits", logits)
-    k, t = int(k), _temperature(temperature)
+    k, t = operator.index(k), _temperature(temperature)
     V = logits.shape[-1]
     if not 1 <= k <= min(V, MAX_K):
         raise ValueError(f"top_logits: k = {k} of {V} classes; 1 to {min(V, MAX_K)} are supported")

@@ -7,6 +7,7 @@ this is the normalisation that needs neither running statistics nor SyncBatchNor
 from __future__ import annotations
 
 import functools
+import operator
 from typing import Optional, Union
 
 import torch
@@ -39,7 +40,7 @@ def _check(x, num_groups, gamma, beta, residual, eps) -> int:
     if x.dtype not in _FLOATS:
         raise TypeError(f"group_norm_act: unsupported dtype {x.dtype}")
     C = shape[-1]
-    groups = int(num_groups)
+    groups = operator.index(num_groups)
     if groups <= 0 or C == 0 or C % groups != 0:
         raise ValueError(f"group_norm_act: {C} channels do not divide into {num_groups} groups")
     if not eps >= 0.0:

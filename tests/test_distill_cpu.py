@@ -21,9 +21,11 @@ def test_top_logits_order():
 def test_top_logits_refusals():
     z = torch.randn(2, 5)
     for kw in (dict(k=0), dict(k=6), dict(k=2, temperature=0.0), dict(k=2, temperature=float("nan")),
-               dict(k=2, temperature=float("inf"))):
+               dict(k=2, temperature=float("inf")), dict(k=2, temperature=1e-9)):
         with pytest.raises(ValueError):
             ops.top_logits(z, **kw)
+    with pytest.raises(TypeError):
+        ops.top_logits(z, 2.5)
     with pytest.raises(TypeError):
         ops.top_logits(z.double(), 2)
     with pytest.raises(TypeError):

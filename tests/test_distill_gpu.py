@@ -43,7 +43,9 @@ def check_top(z, k, t=1.0):
     assert torch.equal(r.isnan(), want.isnan())
     both = ~want.isnan()
     r, want = r[both].double(), want[both]
-    same = r == want   # infinities
+    # infinities, also those that rest's type makes of a sum beyond it: 2^128 (1 - 2^-25) and more round to one in fp32
+    # (the fp32 lowest value over T = 1/4 is -1.36e39), and the comparison is with the rounded sum
+    same = r == torch.where(want.abs() >= 2.0 ** 128 * (1 - 2.0 ** -25), want.sign() * INF, want)
     assert bool((same | ((r - want).abs() <= lse_bound(V) + U * want.abs())).all()), float((r - want).abs().max())
 
 
@@ -231,6 +233,54 @@ def test_distill_loss_remainder_far_below_the_entries():
     r = torch.tensor([8.0, 7.5, 30.0, 8.0], device=DEV)
     row, dz = check_loss(z, v, i, r)
     assert bool(torch.isfinite(row).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t", [1.0, 0.25, 2.0 ** -20])
+def test_masks_of_the_lowest_value_and_tiny_temperatures(dtype, t):
+    """Every class but the entries masked with the type's lowest value; whole rows of it; values near the type's largest."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z = logits(6, 700, dtype, 24)
+    z[0, 5:] = low
+    z[1] = low
+    z[2, 100:] = low / 2
+    z[3] = low / 2
+    z[4, 7] = high / 2
+    z[5, :350], z[5, 350:] = low, -INF
+    i = torch.arange(5, device=DEV).expand(6, 5)
+    v = torch.linspace(1.0, 0.0, 5, device=DEV).expand(6, 5)
+    for k in (3, 5, 400):
+        check_top(z, k, t)
+    # a teacher that leaves nothing to the other classes
+    none = torch.full((6,), -INF, device=DEV)
+    for rest in (None, none):
+        loss, dz, size = exact(z, v, i, rest, t, torch.ones(6, device=DEV))
+        zl = z.clone().requires_grad_(True)
+        row = ops.distill_loss(zl, v, i, rest, t, "none")
+        got, = torch.autograd.grad(row.sum(), zl)
+        r64, big = row.detach().double(), loss.abs() > 1e30
+        # differences of logits over T, rounded in fp32 once: u of their size each
+        lim = t * t * 2 * lse_bound(700) + 8 * U * loss.abs()
+        assert bool((((r64 - loss).abs() <= lim) | big | (r64 == loss)).all()), (r64, loss)
+        half = torch.finfo(dtype).eps / 2
+        assert bool(((got.double() - dz).abs() <= half * dz.abs() + 4 * lse_bound(700) * size + TINY[dtype]).all())
+
+
+def test_offsets_beyond_32_bits():
+    rows, V = 2100, 1 << 20
+    z = torch.zeros((rows, V), device=DEV, dtype=torch.bfloat16)
+    z[-2:] = logits(2, V, torch.bfloat16, 25)
+    v, i, r = ops.top_logits(z, 9, 2.0)
+    small = ops.top_logits(z[-2:].clone(), 9, 2.0)
+    assert torch.equal(v[-2:], small[0]) and torch.equal(i[-2:], small[1]) and torch.equal(r[-2:], small[2])
+    assert torch.equal(i[0], torch.arange(9, device=DEV))
+    zl = z.requires_grad_(True)
+    row = ops.distill_loss(zl, v, i, r, 2.0, "none")
+    dz, = torch.autograd.grad(row.sum(), zl)
+    zs = z.detach()[-2:].clone().requires_grad_(True)
+    rs = ops.distill_loss(zs, small[0], small[1], small[2], 2.0, "none")
+    ds, = torch.autograd.grad(rs.sum(), zs)
+    assert torch.equal(row[-2:], rs) and torch.equal(dz[-2:], ds)
 
 
 def test_distill_loss_nan_and_infinite_rows():

@@ -66,6 +66,8 @@ def test_group_norm_act_refusals():
             ops.group_norm_act(x, **kw)
     with pytest.raises(TypeError):
         ops.group_norm_act(x.double(), 4)
+    with pytest.raises(TypeError):
+        ops.group_norm_act(x, 4.0)
     with pytest.raises(ValueError):
         ops.group_norm_act(torch.randn(8), 4)
 

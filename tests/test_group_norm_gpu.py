@@ -229,6 +229,25 @@ def test_group_norm_act_gradient_subsets_and_parameter_types():
     assert torch.equal(torch.autograd.grad(ops.group_norm_act(x, 4, None, None, r2), r2, dy)[0], dy)
 
 
+@pytest.mark.parametrize("shape", [(1400, 56, 56, 512), (160, 14400, 1024)])
+def test_group_norm_act_offsets_beyond_32_bits(shape):
+    """The last sample lies behind 2^31 elements (in registers, and by row chunks)."""
+    g = torch.Generator(device=DEV).manual_seed(16)
+    one, w, b, _, dy = make((1,) + shape[1:], torch.float16, 17)
+    x = torch.zeros(shape, device=DEV, dtype=torch.float16)
+    x[-1:] = one
+    up = torch.zeros_like(x)
+    up[-1:] = dy
+    xl, wl = x.requires_grad_(True), w.requires_grad_(True)
+    out = ops.group_norm_act(xl, 32, wl, b, None, True)
+    dx, dw = torch.autograd.grad(out, (xl, wl), up)
+    want = exact(one, 32, w, b, None, True, 1e-5, dy)
+    close("out", out[-1:], want["out"])
+    close("dx", dx[-1:], want["dx"])
+    close("dgamma", dw, want["dgamma"])
+    assert not bool(dx[:-1].any())
+
+
 def test_group_norm_act_is_differentiable_once():
     x, w, b, _, dy = make((2, 3, 3, 16), torch.float32, 15)
     xl = x.requires_grad_(True)
