@@ -7,6 +7,7 @@
 #include "common.h"
 
 #include <math.h>
+#include <type_traits>
 
 // Activations (the codes of the Python side).
 enum GnAct : int { GN_NONE = 0, GN_RELU = 1, GN_CAP = 2, GN_SILU = 3 };
@@ -64,6 +65,13 @@ template <typename T, int VEC>
 __device__ __forceinline__ GnVec<T, VEC> gn_ld(const T* p) { return *reinterpret_cast<const GnVec<T, VEC>*>(p); }
 template <typename T, int VEC>
 __device__ __forceinline__ void gn_st(T* p, const GnVec<T, VEC>& v) { *reinterpret_cast<GnVec<T, VEC>*>(p) = v; }
+
+// The vector of a pass over rows, loaded ahead of its use.
+template <typename T, int VEC>
+using GnHeld = typename std::conditional<VEC * sizeof(T) == 16, GnRaw<T>, GnVec<T, VEC>>::type;
+template <typename T, int VEC> __device__ __forceinline__ GnHeld<T, VEC> gn_ld_held(const T* p) {
+  return *reinterpret_cast<const GnHeld<T, VEC>*>(p);
+}
 
 // The channel at a place of a row, where a row may be several positions next to each other.
 __device__ __forceinline__ int gn_channel(int c, int C) {
@@ -163,9 +171,9 @@ __device__ __forceinline__ float gn_silu_slope(float t, const V& w, bool wr, con
 }
 
 // g = dout*act'(z) of a vector; x and res where they stand, c0 the channel of x[0].
-template <int ACT, typename T, int VEC, bool UG>
-__device__ __forceinline__ void gn_grads(float (&g)[VEC], const GnVec<T, VEC>& d, const GnVec<T, VEC>& v, const GnVec<T, VEC>& w,
-                                         bool wr, const GnCoef<VEC, UG>& k, const T* x, const T* res, const GnStat* st,
+template <int ACT, typename T, int VEC, bool UG, typename V>
+__device__ __forceinline__ void gn_grads(float (&g)[VEC], const V& d, const V& v, const V& w, bool wr,
+                                         const GnCoef<VEC, UG>& k, const T* x, const T* res, const GnStat* st,
                                          const float* gamma, const float* beta, int c0, int D, int C, float cap) {
   unsigned on = 0;
   if constexpr (gn_is_relu(ACT)) {
@@ -184,7 +192,7 @@ __device__ __forceinline__ void gn_grads(float (&g)[VEC], const GnVec<T, VEC>& d
   }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
-    const float dy = ElemTraits<T>::to_f32(d.v[e]);
+    const float dy = d.f(e);
     if constexpr (ACT == GN_NONE) g[e] = dy;
     if constexpr (gn_is_relu(ACT)) g[e] = (on >> e) & 1u ? dy : 0.f;
     if constexpr (ACT == GN_SILU) g[e] = dy * gn_silu_slope(v.f(e) - k.mh[UG ? 0 : e], w, wr, k, e);
