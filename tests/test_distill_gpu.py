@@ -58,6 +58,18 @@ def test_top_logits_sizes(rows, V, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,k", [(2, 1), (3, 3), (4, 2), (7, 3), (8, 8), (9, 1), (2048, 100), (2049, 160), (4097, 161), (8193, 160), (16385, 161),
+                                 (32769, 256), (65536, 160), (65537, 160), (65537, 300), (70001, 513)])
+def test_top_logits_few_rows_of_every_way(V, k, dtype):
+    check_top(logits(3, V, dtype, 26), k, 1.0)
+    # runs that are full of candidates: the largest values next to each other, and one in every vector
+    z = logits(3, V, dtype, 27)
+    z[0, V // 2:V // 2 + k] += 40.0
+    z[1, ::max(1, V // k)] += 40.0
+    check_top(z, k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_top_logits_ties_and_specials(dtype):
     low = torch.finfo(dtype).min
     V = 3001
