@@ -663,7 +663,7 @@ distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
 }
 
 // dz of a row: one value for every class, then the entries' own over it (the barrier orders the two writes).  Bound by memory:
-// 8192 x 131072 bf16 855 us = 5.0 TB/s.
+// 8192 x 131072 bf16 785 us = 5.5 TB/s.
 // Rows go from the last to the first: what the forward pass read last is still in the memory-side cache, and a gradient too
 // large to stay there itself passes it by (stream: non-temporal stores; 2047 x 50001 bf16 160 -> 144 us with the forward pass,
 // 8192 x 131072 1250 -> 1212 us).
@@ -809,8 +809,16 @@ PDA_EXPORT int pda_distill_bwd(int dtype, const void* z, long long ld, long long
   if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || V > MAX_CLASSES || K <= 0 || K > MAX_K || !(temperature > 0.0)) return -1;
   const float c = (float)(LOG2E / temperature);
   const int stream = rows * V * (dtype == PDA_F32 ? 4 : 2) > pda_stream_min_bytes();
-  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st,
-                                             (const T*)z, ld, V, indices, idx64, ild, K, c, (const RowStat*)stat, dtop, g,
-                                             gstride, gscale, stream, (T*)dz));
+#define DISTILL_BWD(NT)                                                                                                          \
+  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((distill_bwd_kernel<T, NT>), dim3((unsigned)rows), dim3(NT), 0, st, (const T*)z, ld, V,  \
+                                             indices, idx64, ild, K, c, (const RowStat*)stat, dtop, g, gstride, gscale, stream,   \
+                                             (T*)dz))
+  // long rows: fewer of them at once (256 / 1024 threads: 8192 x 131072 bf16 861 / 778 us, 2047 x 50001 72 / 66,
+  // 32 x 131072 17 / 11, 1024 x 20000 15 / 15)
+  if ((long long)V * (dtype == PDA_F32 ? 4 : 2) < 32 * 1024) {
+    DISTILL_BWD(256)
+  } else {
+    DISTILL_BWD(1024)
+  }
   return pda_check_launch();
 }
