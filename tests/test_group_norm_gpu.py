@@ -183,6 +183,44 @@ def test_group_norm_act_side_of_a_border_is_that_of_fp64(shape, groups, act):
     assert torch.equal((dres != 0)[sure], inside[sure] & (dy != 0)[sure])
 
 
+# as many positions as registers hold
+LONG = [((600, 1500, 32), 4, torch.float32), ((2, 6500, 8), 1, torch.float32), ((2, 6272, 32), 2, torch.float16), ((3, 12999, 8), 1, torch.bfloat16),
+        ((300, 3136, 64), 8, torch.float16), ((2, 6400, 16), 2, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("act", [False, True, 6.0, "silu"])
+@pytest.mark.parametrize("shape,groups,dtype", LONG)
+def test_group_norm_act_long_samples(shape, groups, dtype, act):
+    x, w, b, res, dy = make(shape, dtype, 41, residual=act != 6.0)
+    if act is True or act == 6.0:  # whole vectors and single elements of zero
+        dy[:, 7::50] = 0
+        dy[..., 3] = 0
+    check(x, groups, w, b, res, dy, act)
+
+
+@pytest.mark.parametrize("act", [True, 6.0])
+@pytest.mark.parametrize("shape,groups", [(s, g) for s, g, t in LONG if t == torch.float32])
+def test_group_norm_act_long_samples_all_next_to_a_border(shape, groups, act):
+    """Every element lies next to the border and is decided in fp64; the sums have to follow.  dy is 0 where z is nearer than
+    1e-12.  With g known the bounds are those of sums of g and g xh, each term good to 104 u."""
+    x, w, b, _, dy = make(shape, torch.float32, 43)
+    z = exact(x, groups, w, b, None, False, 1e-5)["out"][0].reshape(shape)
+    border = 0.0 if act is True else 6.0
+    res = (border - z).float()
+    left = z + res.double() - border
+    dy = torch.where(left.abs() > 1e-12, dy, 0.0)
+    leaves = [t.requires_grad_(True) for t in (x, w, b, res)]
+    out = ops.group_norm_act(x, groups, w, b, res, act)
+    dx, dw, db, dres = torch.autograd.grad(out, leaves, dy)
+    g = dy.double() * (left > 0 if act is True else left < 0)
+    assert torch.equal(dres, g.float())
+    # the same gradient through the norm alone
+    want = exact(x, groups, w, b, None, False, 1e-5, g)
+    close("dbeta", db, want["dbeta"])
+    close("dgamma", dw, want["dgamma"])
+    close("dx", dx, want["dx"])
+
+
 def test_group_norm_act_constant_groups_and_nan():
     x = torch.full((2, 6, 6, 16), 3.0, device=DEV)
     w, b = torch.full((16,), 2.0, device=DEV), torch.linspace(-1, 1, 16, device=DEV)
