@@ -745,28 +745,43 @@ row_total_kernel(const float* __restrict__ x, long long n, double scale, float* 
 
 static const double LOG2E = 1.4426950408889634;
 
+// A launch holds fewer than 2^32 threads: rows of one block each go in steps of 2^21.
+constexpr long long ROW_STEP = 1ll << 21;
+template <typename F> static int each_step(long long rows, F launch) {
+  int rc = 0;
+  for (long long r0 = 0; r0 < rows && rc == 0; r0 += ROW_STEP) rc = launch(r0, rows - r0 < ROW_STEP ? rows - r0 : ROW_STEP);
+  return rc;
+}
+static const char* bytes_at(const void* p, long long bytes) { return p ? static_cast<const char*>(p) + bytes : nullptr; }
+static char* bytes_at(void* p, long long bytes) { return static_cast<char*>(p) + bytes; }
+static int size_of(int dtype) { return dtype == PDA_F32 ? 4 : 2; }
+
 PDA_EXPORT int pda_top_logits(int dtype, const void* z, long long ld, long long rows, int V, int K, double temperature,
                               void* values, long long* indices, float* rest, hipStream_t st) {
-  if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || K <= 0 || K > V || K > MAX_K || !(temperature > 0.0)) return -1;
+  if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || V > MAX_CLASSES || K <= 0 || K > V || K > MAX_K || !(temperature > 0.0))
+    return -1;
   const float c = (float)(LOG2E / temperature);
-  const long long bytes = (long long)V * (dtype == PDA_F32 ? 4 : 2);
+  const long long es = size_of(dtype), bytes = V * es;
 #define TOP_LAUNCH(NT, CELLS)                                                                                                  \
-  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, NT, CELLS>), dim3((unsigned)rows), dim3(NT), 0, st,           \
-                                             (const T*)z, ld, V, K, c, temperature, (T*)values, indices, rest))
+  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((top_logits_kernel<T, NT, CELLS>), dim3((unsigned)n), dim3(NT), 0, st,             \
+                                             (const T*)bytes_at(z, r0 * ld * es), ld, V, K, c, temperature,                     \
+                                             (T*)bytes_at(values, r0 * K * es), indices + r0 * K, rest + r0))
   // Threads: enough that the K-th largest of their maxima is close to the K-th largest element (the candidates are about
   // NT log(NT/(NT - K))), few where rows are short, since the steps after the read take as long for any row and other
   // rows' blocks fill the time (256 / 512 threads: 8192 x 20000 fp16 95 / 144 us, 512 x 50000 bf16 18.5 / 20.1,
   // 4096 x 131072 bf16 231 / 211, one row of it 21 / 16).  Short rows: no more runs than they have vectors.
-  if (bytes <= 8 * 1024) {
-    TOP_LAUNCH(256, 2)
-  } else if (K > 160 || bytes > 128 * 1024) {
-    TOP_LAUNCH(512, 8)
-  } else if (bytes <= 32 * 1024) {
-    TOP_LAUNCH(256, 4)
-  } else {
-    TOP_LAUNCH(256, 8)
-  }
-  return pda_check_launch();
+  return each_step(rows, [&](long long r0, long long n) {
+    if (bytes <= 8 * 1024) {
+      TOP_LAUNCH(256, 2)
+    } else if (K > 160 || bytes > 128 * 1024) {
+      TOP_LAUNCH(512, 8)
+    } else if (bytes <= 32 * 1024) {
+      TOP_LAUNCH(256, 4)
+    } else {
+      TOP_LAUNCH(256, 8)
+    }
+    return pda_check_launch();
+  });
 }
 
 template <typename T, int NT>
@@ -792,9 +807,14 @@ PDA_EXPORT int pda_distill_fwd(int dtype, const void* z, long long ld, long long
                                hipStream_t st) {
   if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || V > MAX_CLASSES || K <= 0 || K > MAX_K || !(temperature > 0.0)) return -1;
   if (vdtype != PDA_F32 && vdtype != PDA_F16 && vdtype != PDA_BF16) return -6;
-  int rc = 0;
-  DISTILL_DISPATCH(dtype, rc = launch_distill_fwd<T, 256>(z, ld, rows, V, values, vdtype, vld, indices, idx64, ild, rest, K,
-                                                          temperature, row_loss, stat, dtop, st));
+  int rc = each_step(rows, [&](long long r0, long long n) {
+    const void* zr = bytes_at(z, r0 * ld * size_of(dtype));
+    const void* vr = bytes_at(values, r0 * vld * size_of(vdtype));
+    const void* ir = bytes_at(indices, r0 * ild * (idx64 ? 8 : 4));
+    DISTILL_DISPATCH(dtype, return (launch_distill_fwd<T, 256>(zr, ld, n, V, vr, vdtype, vld, ir, idx64, ild, rest ? rest + r0 : nullptr,
+                                                               K, temperature, row_loss + r0, (RowStat*)stat + r0, dtop + r0 * K, st)));
+    return 0;
+  });
   if (rc == 0 && loss) {
     hipLaunchKernelGGL(row_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, rows, scale, loss);
     rc = pda_check_launch();
@@ -808,17 +828,22 @@ PDA_EXPORT int pda_distill_bwd(int dtype, const void* z, long long ld, long long
                                int gstride, float gscale, void* dz, hipStream_t st) {
   if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || V > MAX_CLASSES || K <= 0 || K > MAX_K || !(temperature > 0.0)) return -1;
   const float c = (float)(LOG2E / temperature);
-  const int stream = rows * V * (dtype == PDA_F32 ? 4 : 2) > pda_stream_min_bytes();
+  const long long es = size_of(dtype);
+  const int stream = rows * V * es > pda_stream_min_bytes();
 #define DISTILL_BWD(NT)                                                                                                          \
-  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((distill_bwd_kernel<T, NT>), dim3((unsigned)rows), dim3(NT), 0, st, (const T*)z, ld, V,  \
-                                             indices, idx64, ild, K, c, (const RowStat*)stat, dtop, g, gstride, gscale, stream,   \
-                                             (T*)dz))
+  DISTILL_DISPATCH(dtype, hipLaunchKernelGGL((distill_bwd_kernel<T, NT>), dim3((unsigned)n), dim3(NT), 0, st,                      \
+                                             (const T*)bytes_at(z, r0 * ld * es), ld, V,                                          \
+                                             bytes_at(indices, r0 * ild * (idx64 ? 8 : 4)), idx64, ild, K, c,                     \
+                                             (const RowStat*)stat + r0, dtop + r0 * K, g + r0 * gstride, gstride, gscale, stream,  \
+                                             (T*)dz + r0 * V))
   // long rows: fewer of them at once (256 / 1024 threads: 8192 x 131072 bf16 861 / 778 us, 2047 x 50001 72 / 66,
   // 32 x 131072 17 / 11, 1024 x 20000 15 / 15)
-  if ((long long)V * (dtype == PDA_F32 ? 4 : 2) < 32 * 1024) {
-    DISTILL_BWD(256)
-  } else {
-    DISTILL_BWD(1024)
-  }
-  return pda_check_launch();
+  return each_step(rows, [&](long long r0, long long n) {
+    if (V * es < 32 * 1024) {
+      DISTILL_BWD(256)
+    } else {
+      DISTILL_BWD(1024)
+    }
+    return pda_check_launch();
+  });
 }

@@ -295,6 +295,26 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(row[-2:], rs) and torch.equal(dz[-2:], ds)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_rows_than_one_launch_holds(dtype):
+    rows, V = (1 << 24) + 7, 6
+    z = torch.zeros((rows, V), device=DEV, dtype=dtype)
+    at = torch.tensor([0, (1 << 21) - 1, 1 << 21, (1 << 23) + 5, 1 << 24, rows - 1], device=DEV)
+    z[at] = logits(6, V, dtype, 28)
+    small = z[at].clone()
+    top, want = ops.top_logits(z, 2, 2.0), ops.top_logits(small, 2, 2.0)
+    for t, w in zip(top, want):
+        assert torch.equal(t[at], w)
+    assert bool((top[1][1] == torch.arange(2, device=DEV)).all())
+    zl, zs = z.requires_grad_(True), (small + 0).requires_grad_(True)
+    weight = torch.arange(rows, device=DEV, dtype=torch.float32)
+    v, i = top[0].flip(0), top[1].flip(0).to(torch.int32)
+    row, few = ops.distill_loss(zl, v, i, top[2], 2.0, "none"), ops.distill_loss(zs, v[at], i[at], top[2][at], 2.0, "none")
+    dz, = torch.autograd.grad(row, zl, weight)
+    ds, = torch.autograd.grad(few, zs, weight[at])
+    assert torch.equal(row[at], few) and torch.equal(dz[at], ds)
+
+
 def test_distill_loss_nan_and_infinite_rows():
     z = logits(4, 300, torch.bfloat16, 11)
     v, i, r = teacher(z, 4, 1.0, 12)
