@@ -430,67 +430,97 @@ PDA_EXPORT int pda_group_norm_plan(int dtype, long long N, long long S, int C, i
   return (int)(want < 1 ? 1 : want > 1024 ? 1024 : want);
 }
 
+// A launch holds fewer than 2^32 threads: samples of `threads` threads each go in steps, one after the other.
+template <typename F> static int gn_each_step(long long N, long long threads, F launch) {
+  const long long step = (1ll << 31) / threads;  // at least 32: 2^20 channels, a wave a group at most
+  if (step < 1) return -1;
+  int rc = 0;
+  for (long long n0 = 0; n0 < N && rc == 0; n0 += step) rc = launch(n0, N - n0 < step ? N - n0 : step);
+  return rc;
+}
+static long long gn_threads(const GnPlan& p, int C, int G, int chunks) {
+  if (chunks == 0) return (long long)p.threads * (C * p.fold / p.W);
+  return 256ll * chunks > 64ll * G ? 256ll * chunks : 64ll * G;
+}
+static const char* gn_at(const void* p, long long bytes) { return p ? static_cast<const char*>(p) + bytes : nullptr; }
+static char* gn_at(void* p, long long bytes) { return p ? static_cast<char*>(p) + bytes : nullptr; }
+
 // chunks: from pda_group_norm_plan, as are those of the backward pass.  part: two fp64 [N][chunks][C] (none at 0 chunks);
 // stats: {fp64 mean, fp64 1/std} [N][G]
-PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x, const void* res, void* out, const float* gamma,
-                                  const float* beta, long long N, long long S, int C, int G, double eps, int act, float cap,
-                                  int chunks, void* part, void* stats, hipStream_t st) {
-  if (!gn_args_ok(N, S, C, G, chunks, act)) return -1;
-  const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, out});
+PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x_, const void* res_, void* out_, const float* gamma,
+                                  const float* beta, long long N_, long long S, int C, int G, double eps, int act, float cap,
+                                  int chunks, void* part_, void* stats_, hipStream_t st) {
+  if (!gn_args_ok(N_, S, C, G, chunks, act)) return -1;
+  const int es = dtype == PDA_F32 ? 4 : 2;
+  const int vec = gn_vec(C, es, {x_, res_, out_});
+  GnPlan p{0, 0, 0};
   if (chunks == 0) {
-    const bool aligned = gn_aligned({x, res, out});
-    const GnPlan p = gn_resident_plan(dtype == PDA_F32 ? 4 : 2, N, S, C, G, false);
-    if (!p.nv || !aligned || N * (C * p.fold / p.W) >= (1ll << 31)) return -1;
-    const GnResidentArgs a{x, res, nullptr, out, nullptr, nullptr, gamma, beta, N, S, C, G, act, eps, cap, (GnStat*)stats,
-                           nullptr, st};
-    return dtype == PDA_F32 ? gn_resident_fwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_fwd<f16>(p, a)
-           : dtype == PDA_BF16 ? gn_resident_fwd<bf16>(p, a) : -6;
+    p = gn_resident_plan(es, N_, S, C, G, false);
+    if (!p.nv || !gn_aligned({x_, res_, out_})) return -1;
   }
-  const int blocks = (int)(N * chunks);
-  GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x, S, C,
-                                             chunks, (GnSums*)part));
-  hipLaunchKernelGGL(gn_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const GnSums*)part, S, C, G, chunks, eps,
-                     (GnStat*)stats);
-  const bool ug = (C / G) % vec == 0;
-  GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_apply_kernel<E, VEC, UG, ACT>), dim3(blocks), dim3(256),
-              0, st, (const E*)x, (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, cap)));
-  return pda_check_launch();
+  return gn_each_step(N_, gn_threads(p, C, G, chunks), [&](long long n0, long long N) -> int {
+    const long long from = n0 * S * C * es;
+    const char *x = gn_at(x_, from), *res = gn_at(res_, from);
+    char* out = gn_at(out_, from);
+    GnStat* stats = (GnStat*)stats_ + n0 * G;
+    GnSums* part = (GnSums*)part_ + n0 * chunks * C;
+    if (chunks == 0) {
+      const GnResidentArgs a{x, res, nullptr, out, nullptr, nullptr, gamma, beta, N, S, C, G, act, eps, cap, stats, nullptr, st};
+      return dtype == PDA_F32 ? gn_resident_fwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_fwd<f16>(p, a)
+             : dtype == PDA_BF16 ? gn_resident_fwd<bf16>(p, a) : -6;
+    }
+    const int blocks = (int)(N * chunks);
+    GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x, S, C,
+                                               chunks, part));
+    hipLaunchKernelGGL(gn_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const GnSums*)part, S, C, G, chunks, eps, stats);
+    const bool ug = (C / G) % vec == 0;
+    GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_apply_kernel<E, VEC, UG, ACT>), dim3(blocks),
+                dim3(256), 0, st, (const E*)x, (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, cap)));
+    return pda_check_launch();
+  });
 }
 
 // part: float2 [N][max(chunks, 1)][C]; ab: float2 [N][G] (none at 0 chunks).  dgamma / dbeta: both or none.
-PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x, const void* res, const void* dout, void* dx, void* dres,
-                                  const float* gamma, const float* beta, const void* stats, long long N, long long S, int C,
-                                  int G, int act, float cap, int chunks, void* part, void* ab, float* dgamma, float* dbeta,
+PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x_, const void* res_, const void* dout_, void* dx_, void* dres_,
+                                  const float* gamma, const float* beta, const void* stats_, long long N_, long long S, int C,
+                                  int G, int act, float cap, int chunks, void* part_, void* ab_, float* dgamma, float* dbeta,
                                   hipStream_t st) {
-  if (!gn_args_ok(N, S, C, G, chunks, act) || (dres && !dx)) return -1;
-  const int vec = gn_vec(C, dtype == PDA_F32 ? 4 : 2, {x, res, dout, dx, dres});
+  if (!gn_args_ok(N_, S, C, G, chunks, act) || (dres_ && !dx_)) return -1;
+  const int es = dtype == PDA_F32 ? 4 : 2;
+  const int vec = gn_vec(C, es, {x_, res_, dout_, dx_, dres_});
+  const float top = act == GN_CAP ? cap : INFINITY;
+  GnPlan p{0, 0, 0};
   if (chunks == 0) {
-    const bool aligned = gn_aligned({x, res, dout, dx, dres});
-    const GnPlan p = gn_resident_plan(dtype == PDA_F32 ? 4 : 2, N, S, C, G, true);
-    if (!p.nv || !aligned || N * (C * p.fold / p.W) >= (1ll << 31)) return -1;
-    const GnResidentArgs a{x, res, dout, nullptr, dx, dres, gamma, beta, N, S, C, G, act, 0.0, act == GN_CAP ? cap : INFINITY, (GnStat*)const_cast<void*>(stats),
-                           dgamma ? (float2*)part : nullptr, st};
-    const int rc = dtype == PDA_F32 ? gn_resident_bwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_bwd<f16>(p, a)
-                   : dtype == PDA_BF16 ? gn_resident_bwd<bf16>(p, a) : -6;
-    if (rc) return rc;
-    if (dgamma)
-      hipLaunchKernelGGL(gn_params_kernel, dim3((C + 3) / 4), dim3(1024), 0, st, (const float2*)part, N, C, dgamma, dbeta);
-    return pda_check_launch();
+    p = gn_resident_plan(es, N_, S, C, G, true);
+    if (!p.nv || !gn_aligned({x_, res_, dout_, dx_, dres_})) return -1;
   }
-  const int blocks = (int)(N * chunks);
-  const bool ug = (C / G) % vec == 0;
-  GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_bwd_partial_kernel<E, VEC, UG, ACT>), dim3(blocks),
-              dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, gamma, beta, (const GnStat*)stats, S, C, G, chunks,
-              act == GN_CAP ? cap : INFINITY, (float2*)part)));
-  hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const float2*)part, gamma, S, C, G, chunks,
-                     (float2*)ab);
-  if (dgamma)
-    hipLaunchKernelGGL(gn_params_kernel, dim3((C + 3) / 4), dim3(1024), 0, st, (const float2*)part, N * chunks, C, dgamma,
-                       dbeta);
-  if (dx)
-    GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_bwd_apply_kernel<E, VEC, UG, ACT>), dim3(blocks),
-                dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, (E*)dx, (E*)dres, gamma, beta,
-                (const GnStat*)stats, (const float2*)ab, S, C, G, chunks,
-                act == GN_CAP ? cap : INFINITY)));
+  const int rc = gn_each_step(N_, gn_threads(p, C, G, chunks), [&](long long n0, long long N) -> int {
+    const long long from = n0 * S * C * es;
+    const char *x = gn_at(x_, from), *res = gn_at(res_, from), *dout = gn_at(dout_, from);
+    char *dx = gn_at(dx_, from), *dres = gn_at(dres_, from);
+    const GnStat* stats = (const GnStat*)stats_ + n0 * G;
+    float2* part = (float2*)part_ + n0 * (chunks ? chunks : 1) * C;
+    if (chunks == 0) {
+      const GnResidentArgs a{x, res, dout, nullptr, dx, dres, gamma, beta, N, S, C, G, act, 0.0, top, const_cast<GnStat*>(stats),
+                             dgamma ? part : nullptr, st};
+      return dtype == PDA_F32 ? gn_resident_bwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_bwd<f16>(p, a)
+             : dtype == PDA_BF16 ? gn_resident_bwd<bf16>(p, a) : -6;
+    }
+    float2* ab = (float2*)ab_ + n0 * G;
+    const int blocks = (int)(N * chunks);
+    const bool ug = (C / G) % vec == 0;
+    GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_bwd_partial_kernel<E, VEC, UG, ACT>), dim3(blocks),
+                dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, gamma, beta, stats, S, C, G, chunks, top, part)));
+    hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const float2*)part, gamma, S, C, G, chunks,
+                       ab);
+    if (dx)
+      GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_bwd_apply_kernel<E, VEC, UG, ACT>), dim3(blocks),
+                  dim3(256), 0, st, (const E*)x, (const E*)res, (const E*)dout, (E*)dx, (E*)dres, gamma, beta, stats,
+                  (const float2*)ab, S, C, G, chunks, top)));
+    return pda_check_launch();
+  });
+  if (rc || !dgamma) return rc;
+  hipLaunchKernelGGL(gn_params_kernel, dim3((C + 3) / 4), dim3(1024), 0, st, (const float2*)part_, N_ * (chunks ? chunks : 1), C,
+                     dgamma, dbeta);
   return pda_check_launch();
 }

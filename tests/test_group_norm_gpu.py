@@ -286,6 +286,24 @@ def test_group_norm_act_offsets_beyond_32_bits(shape):
     assert not bool(dx[:-1].any())
 
 
+@pytest.mark.parametrize("shape,groups,dtype", [(((1 << 25) + 3, 16), 2, torch.float16), (((1 << 24) + 3, 2, 5), 1, torch.bfloat16)])
+def test_group_norm_act_more_samples_than_one_launch_holds(shape, groups, dtype):
+    x = torch.ones(shape, device=DEV, dtype=dtype)
+    at = torch.tensor([0, 1, (1 << 21) - 1, 1 << 21, 1 << 23, (1 << 24) - 1, 1 << 24, shape[0] - 1], device=DEV)
+    some, w, b, _, dy = make((8,) + shape[1:], dtype, 29)
+    x[at] = some
+    full = torch.zeros(shape, device=DEV, dtype=dtype)
+    full[at] = dy
+    x.requires_grad_(True), some.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+    out, few = ops.group_norm_act(x, groups, w, b, None, "silu"), ops.group_norm_act(some, groups, w, b, None, "silu")
+    got, want = torch.autograd.grad(out, (x, w, b), full), exact(some, groups, w, b, None, "silu", 1e-5, dy)
+    close("out", out[at].detach(), want["out"])
+    close("few", few.detach(), want["out"])
+    close("dx", got[0][at], want["dx"])
+    close("dgamma", got[1], want["dgamma"])
+    close("dbeta", got[2], want["dbeta"])
+
+
 def test_group_norm_act_is_differentiable_once():
     x, w, b, _, dy = make((2, 3, 3, 16), torch.float32, 15)
     xl = x.requires_grad_(True)
