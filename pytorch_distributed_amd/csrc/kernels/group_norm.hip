@@ -264,25 +264,28 @@ gn_bwd_finalize_kernel(const float2* __restrict__ part, const float* __restrict_
 }
 
 // dgamma_c, dbeta_c: the column sums of part [rows][C].  A block takes 4 channels with 256 lanes of rows each: with one
-// block a channel group the walk over the rows (thousands at large batch) has to be short.
+// block a channel group the walk over the rows (thousands at large batch) has to be short.  Many rows are summed in two
+// steps: blockIdx.y takes `span` rows and leaves their sums in the first of them, which no other block reads; the second
+// step (dbeta given) takes those, `step` rows apart.
 __global__ void __launch_bounds__(1024)
-gn_params_kernel(const float2* __restrict__ part, long long rows, int C, float* __restrict__ dgamma,
+gn_params_kernel(float2* part, long long rows, long long span, long long step, int C, float* __restrict__ dgamma,
                  float* __restrict__ dbeta) {
   __shared__ double ra[16][4], rb[16][4];
   const int cl = threadIdx.x & 3, lane = threadIdx.x >> 2;
   const int c = blockIdx.x * 4 + cl;
+  const long long r0 = blockIdx.y * span, r1 = r0 + span < rows ? r0 + span : rows, row = step * C;
   double a = 0.0, b = 0.0;
   if (c < C) {
-    long long r = lane;
-    for (; r + 768 < rows; r += 1024) {
+    long long r = r0 + lane;
+    for (; r + 768 < r1; r += 1024) {
       float2 v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = part[(r + u * 256) * C + c];
+      for (int u = 0; u < 4; ++u) v[u] = part[(r + u * 256) * row + c];
 #pragma unroll
       for (int u = 0; u < 4; ++u) { a += (double)v[u].x; b += (double)v[u].y; }
     }
-    for (; r < rows; r += 256) {
-      const float2 v = part[r * C + c];
+    for (; r < r1; r += 256) {
+      const float2 v = part[r * row + c];
       a += (double)v.x;
       b += (double)v.y;
     }
@@ -298,8 +301,12 @@ gn_params_kernel(const float2* __restrict__ part, long long rows, int C, float* 
   if (threadIdx.x < 4 && c < C) {
 #pragma unroll
     for (int w = 1; w < 16; ++w) { a += ra[w][cl]; b += rb[w][cl]; }
-    dbeta[c] = (float)a;
-    dgamma[c] = (float)b;
+    if (dbeta) {
+      dbeta[c] = (float)a;
+      dgamma[c] = (float)b;
+    } else {
+      part[r0 * row + c] = make_float2((float)a, (float)b);
+    }
   }
 }
 
@@ -520,7 +527,16 @@ PDA_EXPORT int pda_group_norm_bwd(int dtype, const void* x_, const void* res_, c
     return pda_check_launch();
   });
   if (rc || !dgamma) return rc;
-  hipLaunchKernelGGL(gn_params_kernel, dim3((C + 3) / 4), dim3(1024), 0, st, (const float2*)part_, N_ * (chunks ? chunks : 1), C,
-                     dgamma, dbeta);
+  // two steps where one block a channel group would walk far (2^20 x 16 channels 1280 us in one)
+  long long rows = N_ * (chunks ? chunks : 1), step = 1;
+  const dim3 grid((C + 3) / 4), block(1024);
+  if (rows > 4096) {
+    const long long span = rows > 512 * 1024ll ? (rows + 1023) / 1024 : 512, parts = (rows + span - 1) / span;
+    hipLaunchKernelGGL(gn_params_kernel, dim3(grid.x, (unsigned)parts), block, 0, st, (float2*)part_, rows, span, step, C, nullptr,
+                       nullptr);
+    rows = parts;
+    step = span;
+  }
+  hipLaunchKernelGGL(gn_params_kernel, grid, block, 0, st, (float2*)part_, rows, rows, step, C, dgamma, dbeta);
   return pda_check_launch();
 }

@@ -304,6 +304,12 @@ def test_group_norm_act_more_samples_than_one_launch_holds(shape, groups, dtype)
     close("dbeta", got[2], want["dbeta"])
 
 
+@pytest.mark.parametrize("shape,groups", [((4096, 1, 16), 2), ((4097, 1, 16), 2), ((5000, 2, 2, 30), 3), ((600000, 24), 3)])
+def test_group_norm_act_parameter_sums_over_many_samples(shape, groups):
+    x, w, b, _, dy = make(shape, torch.float32, 44)
+    check(x, groups, w, b, None, dy, "silu")
+
+
 def test_group_norm_act_is_differentiable_once():
     x, w, b, _, dy = make((2, 3, 3, 16), torch.float32, 15)
     xl = x.requires_grad_(True)
