@@ -132,15 +132,21 @@ def _backward(ctx, dout):
             means = N * groups * 2 if chunks else 0
             work = torch.empty((sums + means,), device=x.device, dtype=torch.float32)
             if params:
-                dg, db = (torch.empty((C,), device=x.device, dtype=torch.float32) for _ in range(2))
+                dg = torch.empty((C,), device=x.device, dtype=torch.float32)
+                db = torch.empty((C,), device=x.device, dtype=torch.float32)
             at = work.data_ptr()
             _lib.check(l.pda_group_norm_bwd(code, x.data_ptr(), _lib.ptr(residual), dout.data_ptr(), _lib.ptr(dx),
                                             _lib.ptr(dres) if act else 0, _lib.ptr(ga), _lib.ptr(be), stats.data_ptr(), N, S, C,
                                             groups, act, cap, chunks, at, at + 4 * sums, _lib.ptr(dg), _lib.ptr(db),
                                             _lib.stream()), "pda_group_norm_bwd")
-        if params:
-            dg = dg.to(gamma.dtype) if want_g else None
-            db = db.to(beta.dtype) if want_b else None
+        if not want_g:
+            dg = None
+        elif gamma.dtype is not torch.float32:
+            dg = dg.to(gamma.dtype)
+        if not want_b:
+            db = None
+        elif beta.dtype is not torch.float32:
+            db = db.to(beta.dtype)
     return dx if want_dx else None, dg, db, dres, None, None, None, None
 
 
