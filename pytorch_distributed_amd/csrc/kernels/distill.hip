@@ -68,7 +68,7 @@ struct FastSum {
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, z[e]);
     if (top > m) {
-      const float mc2 = top * c;
+      const float mc2 = fmaxf(top * c, -FLT_MAX);  // (finite: a thread that meets masks first goes on from its next maximum)
       s *= s == 0.f ? 0.f : __builtin_amdgcn_exp2f(mc - mc2);
       m = top;
       mc = mc2;
@@ -339,9 +339,9 @@ top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, 
     float base = -FLT_MAX, sum = 0.f;
 #pragma unroll
     for (int q = 0; q < CELLS; ++q) {
-      // (a sum of 0: infinities below, or the lowest fp32 number; the maximum is a number)
+      // (a sum of 0: -inf alone)
       const bool some = (int)threadIdx.x + NT * q * per < nv;
-      const bool again = some && (!(cell[q].s < INFINITY) || cell[q].s == 0.f || !(cell[q].m < low));
+      const bool again = some && (!(cell[q].s < INFINITY) || !((cell[q].s == 0.f ? -INFINITY : cell[q].m) < low));
       mask[q] = __ballot(again);
       own += __popcll(mask[q]);
       if (!some || again) cell[q] = MaxSum{-FLT_MAX, 0.f};

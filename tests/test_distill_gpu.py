@@ -278,6 +278,33 @@ def test_masks_of_the_lowest_value_and_tiny_temperatures(dtype, t):
         assert bool(((got.double() - dz).abs() <= half * dz.abs() + 4 * lse_bound(700) * size + TINY[dtype]).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [2000, 50001, 131072])
+@pytest.mark.parametrize("lowest", [False, True])
+def test_masked_classes(V, lowest, dtype):
+    """Whole runs of a row are masked: its front, its end, most of it, all but fewer than k, everything."""
+    mask = torch.finfo(dtype).min if lowest else -INF
+    z = logits(6, V, dtype, 30)
+    z[0, :V // 2] = mask
+    z[1, V - V // 3:] = mask
+    z[2, torch.rand(V, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) < 0.95] = mask
+    z[3, 10:] = mask
+    z[4, :V - 10] = mask
+    z[5] = mask
+    check_top(z, 20, 2.0)
+    z = z[:5]
+    v, i, _ = teacher(logits(5, V, dtype, 32), 4, 2.0, 33)
+    some = ~(z.gather(-1, i) == mask).any(-1)  # (an entry that the student masks: its loss is infinite, or of 1e38)
+    rest = torch.zeros(5, device=DEV)
+    loss, dz, size = exact(z, v, i, rest, 2.0, torch.ones(5, device=DEV))
+    zl = z.clone().requires_grad_(True)
+    row = ops.distill_loss(zl, v, i, rest, 2.0, "none")
+    got, = torch.autograd.grad(row.sum(), zl)
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((row.detach().double() - loss).abs() <= 4 * 2 * lse_bound(V) + 8 * U * loss.abs())[some].all()), (row, loss)
+    assert bool(((got.double() - dz).abs() <= half * dz.abs() + 4 * lse_bound(V) * size + TINY[dtype])[some].all())
+
+
 def test_offsets_beyond_32_bits():
     rows, V = 2100, 1 << 20
     z = torch.zeros((rows, V), device=DEV, dtype=torch.bfloat16)
