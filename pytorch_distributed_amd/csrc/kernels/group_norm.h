@@ -15,6 +15,31 @@ constexpr bool gn_is_relu(int act) { return act == GN_RELU || act == GN_CAP; }
 
 struct GnStat { double mean, rstd; };
 
+// Statistics of a group of m elements, from fp64 sums A of d = x - p and B of d^2.  B/m - (A/m)^2 as such would leave 2^-53 mean^2,
+// which is more than the variance of values that are nearly alike.
+// fp32: p is the group's first element (its first channel at the sample's first position), taken off each value in fp64, and
+// (p - mean)^2 is at most m var: the variance is good to some m 2^-53 of itself wherever the mean lies.
+// 16 bits: p is 0 (subtracting costs 400x28x28x128 fp16, D = 4, 60 us for 49).  All terms are multiples of q^2, q the last place
+// of the least |x|: where m x^2 <= 2^53 q^2 for the largest one, A and B are exact, and with c = A/m as rounded and e = A - m c,
+// m var = B - c A - c e, each difference rounded once.  Where that fails, then (m < 2^27) the least |x| is below a quarter of the
+// largest, x^2 is at most 4 m var, and 2^-53 of it no more than above.
+struct GnPair { double a, b; };
+template <typename T> __device__ __forceinline__ void gn_add(GnPair& s, float x, double p) {
+  const double d = sizeof(T) == 4 ? (double)x - p : (double)x;
+  s.a += d;
+  s.b += d * d;
+}
+__device__ __forceinline__ GnStat gn_stat(const GnPair& s, double p, double m, double im, double eps) {
+  const double c = s.a * im, e = fma(-m, c, s.a);
+  double var = (fma(-c, s.a, s.b) - c * e) * im;
+  var = var < 0.0 ? 0.0 : var;  // (a NaN stays one)
+  return GnStat{p + fma(e, im, c), 1.0 / sqrt(var + eps)};
+}
+// fp32: the first element of channel c's group; xn: the sample.
+template <typename T> __device__ __forceinline__ double gn_first(const T* xn, int c, int D) {
+  return sizeof(T) == 4 ? (double)ElemTraits<T>::to_f32(xn[c / D * D]) : 0.0;
+}
+
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) GnVec {
   T v[VEC];
   __device__ __forceinline__ float f(int e) const { return ElemTraits<T>::to_f32(v[e]); }

@@ -1,9 +1,8 @@
 // Group norm with an optional residual and activation, channels last: x [N][S][C], C = G groups of D channels.  The formulas
 // are those of group_norm.h.
 //
-// Statistics are sums of x and x^2 in fp64 (the products are exact there, and a mean far from zero may be taken off
-// afterwards) and are kept in fp64: a value next to an activation's border is placed by them.  The element passes take mu as
-// an fp32 pair (hi subtracted from x, lo folded into the shift).
+// Statistics are fp64 sums (gn_stat) and are kept in fp64: a value next to an activation's border is placed by them.  The element
+// passes take mu as an fp32 pair (hi subtracted from x, lo folded into the shift).
 //
 // Memory-bound throughout: the work is split over (sample, row chunk), a thread owns one vector of channels and walks
 // rows, so the per-channel coefficients stay in registers; 2048 blocks of two or four rows in flight a thread measured
@@ -28,34 +27,30 @@ struct GnGeom {
   }
 };
 
-// Sum of x and of x^2.
-struct GnSums { double a, b; };
-
 // Per-channel sums of one row chunk -> part[n][chunk][c].
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
-gn_partial_kernel(const T* __restrict__ x, long long S, int C, int chunks, GnSums* __restrict__ part) {
-  __shared__ GnSums sm[256 * VEC];
+gn_partial_kernel(const T* __restrict__ x, long long S, int C, int G, int chunks, GnPair* __restrict__ part) {
+  __shared__ GnPair sm[256 * VEC];
   const int n = blockIdx.x / chunks, ch = blockIdx.x % chunks;
   const long long r0 = S * ch / chunks, r1 = S * (ch + 1) / chunks;
-  const int vpr = C / VEC;
+  const int vpr = C / VEC, D = C / G;
   const GnGeom g(vpr);
   const T* xn = x + (long long)n * S * C;
   for (int c0 = 0; c0 < vpr; c0 += g.VT) {
     const int vec = c0 + g.col;
     const bool active = g.rl < g.RS && vec < vpr;
-    GnSums s[VEC];
+    GnPair s[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) s[e] = GnSums{0.0, 0.0};
+    for (int e = 0; e < VEC; ++e) s[e] = GnPair{0.0, 0.0};
     if (active) {
       const T* p = xn + (long long)vec * VEC;
+      double first[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) first[e] = gn_first(xn, vec * VEC + e, D);
       const auto add = [&](const GnHeld<T, VEC>& v) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const double f = (double)v.f(e);
-          s[e].a += f;
-          s[e].b += f * f;
-        }
+        for (int e = 0; e < VEC; ++e) gn_add<T>(s[e], v.f(e), first[e]);
       };
       long long r = r0 + g.rl;
       for (; r + 3 * g.RS < r1; r += 4 * g.RS) {
@@ -85,7 +80,7 @@ gn_partial_kernel(const T* __restrict__ x, long long S, int C, int chunks, GnSum
       __syncthreads();
     }
     if (active && g.rl == 0) {
-      GnSums* o = part + (long long)blockIdx.x * C + (long long)vec * VEC;
+      GnPair* o = part + (long long)blockIdx.x * C + (long long)vec * VEC;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) o[e] = s[e];
     }
@@ -93,24 +88,23 @@ gn_partial_kernel(const T* __restrict__ x, long long S, int C, int chunks, GnSum
 }
 
 // One wave per (sample, group): chunks x D sums -> {mu, r} in fp64.
+template <typename T>
 __global__ void __launch_bounds__(64)
-gn_finalize_kernel(const GnSums* __restrict__ part, long long S, int C, int G, int chunks, double eps,
+gn_finalize_kernel(const T* __restrict__ x, const GnPair* __restrict__ part, long long S, int C, int G, int chunks, double eps,
                    GnStat* __restrict__ stats) {
   const int D = C / G;
   const int n = blockIdx.x / G, g = blockIdx.x % G;
-  const GnSums* p = part + (long long)n * chunks * C + (long long)g * D;
+  const GnPair* p = part + (long long)n * chunks * C + (long long)g * D;
   const long long pairs = (long long)chunks * D;
   double a = 0.0, b = 0.0;
   for (long long j = threadIdx.x; j < pairs; j += 64) {
-    const GnSums v = p[(j / D) * C + j % D];
+    const GnPair v = p[(j / D) * C + j % D];
     a += v.a;
     b += v.b;
   }
   const double m = (double)S * D;
-  const double mean = wave_sum_f64(a) / m;
-  double var = wave_sum_f64(b) / m - mean * mean;
-  var = var < 0.0 ? 0.0 : var;  // (a NaN stays one)
-  if (threadIdx.x == 0) stats[blockIdx.x] = GnStat{mean, 1.0 / sqrt(var + eps)};
+  const GnPair s{wave_sum_f64(a), wave_sum_f64(b)};
+  if (threadIdx.x == 0) stats[blockIdx.x] = gn_stat(s, gn_first(x + (long long)n * S * C, g * D, D), m, 1.0 / m, eps);
 }
 
 template <typename T, int VEC, bool UG, int ACT>
@@ -470,16 +464,17 @@ PDA_EXPORT int pda_group_norm_fwd(int dtype, const void* x_, const void* res_, v
     const char *x = gn_at(x_, from), *res = gn_at(res_, from);
     char* out = gn_at(out_, from);
     GnStat* stats = (GnStat*)stats_ + n0 * G;
-    GnSums* part = (GnSums*)part_ + n0 * chunks * C;
+    GnPair* part = (GnPair*)part_ + n0 * chunks * C;
     if (chunks == 0) {
       const GnResidentArgs a{x, res, nullptr, out, nullptr, nullptr, gamma, beta, N, S, C, G, act, eps, cap, stats, nullptr, st};
       return dtype == PDA_F32 ? gn_resident_fwd<float>(p, a) : dtype == PDA_F16 ? gn_resident_fwd<f16>(p, a)
              : dtype == PDA_BF16 ? gn_resident_fwd<bf16>(p, a) : -6;
     }
     const int blocks = (int)(N * chunks);
-    GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x, S, C,
+    GN_DISPATCH(dtype, vec, hipLaunchKernelGGL((gn_partial_kernel<E, VEC>), dim3(blocks), dim3(256), 0, st, (const E*)x, S, C, G,
                                                chunks, part));
-    hipLaunchKernelGGL(gn_finalize_kernel, dim3((int)(N * G)), dim3(64), 0, st, (const GnSums*)part, S, C, G, chunks, eps, stats);
+    GN_DISPATCH(dtype, 1, hipLaunchKernelGGL((gn_finalize_kernel<E>), dim3((int)(N * G)), dim3(64), 0, st, (const E*)x,
+                                             (const GnPair*)part, S, C, G, chunks, eps, stats));
     const bool ug = (C / G) % vec == 0;
     GN_DISPATCH(dtype, vec, GN_DISPATCH_ACT(act, ug, hipLaunchKernelGGL((gn_apply_kernel<E, VEC, UG, ACT>), dim3(blocks),
                 dim3(256), 0, st, (const E*)x, (const E*)res, (E*)out, gamma, beta, (const GnStat*)stats, S, C, G, chunks, cap)));

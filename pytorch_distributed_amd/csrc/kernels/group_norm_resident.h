@@ -100,8 +100,6 @@ template <typename V> __device__ __forceinline__ void gn_channel_totals(V* buf, 
   __syncthreads();
 }
 
-struct GnPair { double a, b; };
-
 // Sums over every group of the slab: s[e] of every thread that is on -> s[e] of the group of slot e (UG: one slot).
 template <int VEC, bool UG>
 __device__ __forceinline__ void gn_group_totals(GnPair (&s)[UG ? 1 : VEC], double* lds, int W, int D, int C, int fold, int RS,
@@ -222,40 +220,33 @@ gn_resident_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (in(i)) v[i] = gn_ld_raw<T>(x + at(i) + off);
-  // Sums of x and of x^2 in fp64: the products are exact there, a mean far from zero may be taken off afterwards, and the side
-  // of an activation's border on which an element lies can be decided by what comes out (a sum of squares in fp32, joined
-  // in fp64, put one element of 300 million on the wrong one).
+  // Sums in fp64: a spread far below the mean is kept, and the side of an activation's border on which an element lies can be
+  // decided by what comes out (a sum of squares in fp32, joined in fp64, put one element of 300 million on the wrong one).
+  double first[NG];
   GnPair tot[NG];
 #pragma unroll
-  for (int i = 0; i < NG; ++i) tot[i] = GnPair{0.0, 0.0};
+  for (int i = 0; i < NG; ++i) {
+    first[i] = gn_first(x + (long long)n * S * row, gn_channel(c0 + col * VEC + i, C), D);
+    tot[i] = GnPair{0.0, 0.0};
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (in(i))
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const double f = (double)v[i].f(e);
-        tot[UG ? 0 : e].a += f;
-        tot[UG ? 0 : e].b += f * f;
-      }
+      for (int e = 0; e < VEC; ++e) gn_add<T>(tot[UG ? 0 : e], v[i].f(e), first[UG ? 0 : e]);
   gn_group_totals<VEC, UG>(tot, lds, W, D, C, fold, RS, col, rl, on, shuffles);
-  const double im = 1.0 / ((double)S * fold * D);
-  float mh[NG];
-#pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    tot[i].a *= im;
-    mh[i] = (float)tot[i].a;
-  }
+  const double m = (double)S * fold * D, im = 1.0 / m;
   if (!on) return;
-  float sc[VEC], sh[VEC];
+  float mh[NG], sc[VEC], sh[VEC];
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
-    const double mean = tot[i].a, ml = mean - (double)mh[i];
-    double var = tot[i].b * im - mean * mean;
-    var = var < 0.0 ? 0.0 : var;  // (a NaN stays one)
-    const double r = 1.0 / sqrt(var + eps);
+    const GnStat st = gn_stat(tot[i], first[i], m, im, eps);
+    const double r = st.rstd;
+    mh[i] = (float)st.mean;
+    const double ml = st.mean - (double)mh[i];
     if (rl == 0) {
       const int c = c0 + col * VEC + i;  // the thread of a group's first channel writes its statistics
-      if (c < C && c % D == 0) stats[(long long)n * G + c / D] = GnStat{mean, r};
+      if (c < C && c % D == 0) stats[(long long)n * G + c / D] = st;
     }
 #pragma unroll
     for (int e = UG ? 0 : i; e < (UG ? VEC : i + 1); ++e) {

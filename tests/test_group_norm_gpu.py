@@ -147,6 +147,30 @@ def test_group_norm_act_mean_far_from_zero(offset):
     check(x, 4, w, b, None, dy, "silu")
 
 
+@pytest.mark.parametrize("shape,groups", [((2, 20, 20, 32), 4), ((2, 20, 20, 8), 4), ((3, 6, 6, 58), 2), ((2, 14, 14, 48), 8),
+                                          ((2, 13, 7, 3), 1), ((2, 120, 120, 24), 3), ((2, 120, 120, 24), 12),
+                                          ((2, 56, 56, 64), 1)])
+@pytest.mark.parametrize("dtype,offset,spread", [(torch.float32, 123457.0, 1.0), (torch.float32, -2000003.0, 1.0),
+                                                 (torch.float16, 40000.0, 156.25), (torch.bfloat16, -189.0 * 2 ** 25, 2.0 ** 26)])
+def test_group_norm_act_spread_far_below_the_mean(shape, groups, dtype, offset, spread):
+    """Values whose spread is a small part of their mean, and none at all in the last sample (r = 1/sqrt(eps) there).  With
+    differences to one of a group's m elements, p, a variance is off by some 2^-53 ((p - mean)^2 + spread^2), and (p - mean)^2 is at
+    most m <= 14400 * 64 times spread^2: 2^-33 of it, far inside the bounds.  The oracle's values have the offset taken off
+    first, which is exact in 64 bits."""
+    x, w, b, _, dy = make(shape, dtype, 51)
+    x = ((x.float() * 8).round() / 8 * spread + offset).to(dtype)
+    x[-1] = offset
+    left = x.double() - offset
+    assert bool(torch.isfinite(x).all()) and not bool(left[-1].any())
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    for act in (False, "silu"):
+        out = ops.group_norm_act(x, groups, w, b, None, act)
+        want = exact(left, groups, w, b, None, act, 1e-5, dy)
+        close("out", out.detach(), want["out"])
+        for n, t in zip(("dx", "dgamma", "dbeta"), torch.autograd.grad(out, leaves, dy)):
+            close(n, t, want[n])
+
+
 def test_group_norm_act_borders_of_the_activation():
     """res such that z is the rounding of an fp32 number, to either side of 0.  x is a multiple of 2^-6 below 4 in size: sums of
     four such and of their squares are exact in fp32, so the statistics are those of fp64, good to 1e-12."""
