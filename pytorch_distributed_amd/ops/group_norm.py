@@ -167,7 +167,7 @@ def group_norm_act_ref(x, groups, gamma, beta, residual, act, cap, eps):
     if act == 3:
         z = F.silu(z)
     elif act:
-        z = torch.relu(z) if act == 1 else torch.clamp(z, 0.0, cap)
+        z = torch.relu(z) if act == 1 else F.hardtanh(z, 0.0, cap)  # (clamp's gradient counts its borders as inside)
     return z.to(x.dtype)
 
 

@@ -132,3 +132,16 @@ def test_group_norm_resnet_layers_one_by_one():
     torch.testing.assert_close(got, want, rtol=1e-3, atol=1e-4)
     for a, b in zip(gg, gw):
         torch.testing.assert_close(a, b, rtol=1e-2, atol=1e-3 * float(b.abs().max()))
+
+
+@pytest.mark.parametrize("act,border", [(True, 0.0), (6.0, 0.0), (6.0, 6.0), (0.5, 0.5)])
+def test_group_norm_act_no_gradient_on_a_border(act, border):
+    """z exactly on a border (gamma 0, beta or the residual the border): no gradient comes through, as in relu and relu6."""
+    g = torch.Generator().manual_seed(9)
+    x, dy = torch.randn(2, 5, 8, generator=g), torch.randn(2, 5, 8, generator=g)
+    for by_beta in (True, False):
+        beta, res = (border, 0.0) if by_beta else (0.0, border)
+        leaves = [t.requires_grad_(True) for t in (x.clone(), torch.zeros(8), torch.full((8,), beta), torch.full((2, 5, 8), res))]
+        out = ops.group_norm_act(leaves[0], 2, leaves[1], leaves[2], leaves[3], act)
+        assert torch.equal(out, torch.full_like(out, border))
+        assert not any(bool(t.any()) for t in torch.autograd.grad(out, leaves, dy))

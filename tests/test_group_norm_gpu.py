@@ -188,6 +188,20 @@ def test_group_norm_act_borders_of_the_activation():
     assert torch.equal((dres != 0)[sure], (left > 0)[sure] & (dy != 0)[sure])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,groups", [((2, 6, 6, 32), 4), ((2, 9, 11, 58), 29), ((1, 120, 120, 24), 3)])
+@pytest.mark.parametrize("act,border", [(True, 0.0), (6.0, 0.0), (6.0, 6.0), (0.5, 0.5)])
+def test_group_norm_act_no_gradient_on_a_border(act, border, shape, groups, dtype):
+    x, _, _, _, dy = make(shape, dtype, 52)
+    for by_beta in (True, False):
+        beta, res = (border, 0.0) if by_beta else (0.0, border)
+        leaves = [t.requires_grad_(True) for t in (x.clone(), torch.zeros(shape[-1], device=DEV),
+                                                   torch.full((shape[-1],), beta, device=DEV), torch.full_like(x, res))]
+        out = ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], leaves[3], act)
+        assert torch.equal(out, torch.full_like(out, border))
+        assert not any(bool(t.any()) for t in torch.autograd.grad(out, leaves, dy))
+
+
 @pytest.mark.parametrize("shape,groups", [((2, 300, 8), 2), ((3, 28, 28, 64), 8), ((2, 56, 56, 32), 16), ((2, 15000, 8), 2),
                                           ((2, 9, 11, 58), 29)])
 @pytest.mark.parametrize("act", [True, 6.0])
