@@ -155,16 +155,18 @@ def distill_loss_ref(logits, values, indices, rest, temperature, reduction):
     p = torch.zeros((z.shape[0], V + 1), dtype=torch.float64, device=z.device).scatter_add_(1, slot, tau.exp() / norm)[:, :V]
     taken = torch.zeros((z.shape[0], V + 1), dtype=torch.bool, device=z.device).scatter_(1, slot, True)[:, :V]
     # a row without entries is not read
-    logq = torch.log_softmax(torch.where(keep, z, torch.zeros_like(z)) / temperature, dim=1)
+    u = torch.where(keep, z, torch.zeros_like(z)) / temperature
+    logq = torch.log_softmax(u, dim=1)
     on = p != 0
     terms = torch.where(on, p * (torch.where(on, p, 1.0).log() - torch.where(on, logq, 0.0)), 0.0)
     loss = terms.sum(1)
     if rest is not None:
         pr = (left.exp() / norm)[:, 0]
         has = (pr != 0) & some
-        open_ = has & ~taken.all(1)
+        # nothing left outside the entries: log 0, whose gradient is that of the normaliser alone
+        open_ = has & (~taken & (logq != -math.inf)).any(1)
         lt = torch.logsumexp(torch.where(open_[:, None], logq.masked_fill(taken, -math.inf), logq), dim=1)
-        lt = torch.where(has & ~open_, -math.inf, lt)
+        lt = torch.where(has & ~open_, -math.inf - torch.logsumexp(u, dim=1), lt)
         loss = loss + torch.where(has, pr * (torch.where(has, pr, 1.0).log() - torch.where(has, lt, 0.0)), 0.0)
     loss = torch.where(some, loss, 0.0) * temperature ** 2
     if reduction == "none":

@@ -109,6 +109,32 @@ def test_distill_loss_rows(with_rest):
         assert abs(float(num) - float(gz[k, c])) < h * h + 2.0 ** -24 * 8 / h
 
 
+def closed_rows():
+    """Rows whose student leaves nothing to the classes that are not entries while the teacher's rest has a share: the loss is inf, the
+    gradient T (q - p) at the entries and zero elsewhere."""
+    inf = math.inf
+    z = torch.tensor([[1.0, 2.0, -inf, -inf], [0.5, -inf, 3.0, -inf], [0.3, -1.0, 2.0, 0.7], [0.1, 0.2, 0.3, 0.4]])
+    v = torch.tensor([[0.2, 0.4, 0.0, 0.0], [1.0, 0.1, 0.3, 0.0], [0.1, 0.2, 0.3, 0.4], [0.1, 0.2, 0.3, 0.0]])
+    i = torch.tensor([[0, 1, -1, -1], [0, 1, 2, -1], [0, 1, 2, 3], [0, 1, 2, -1]])
+    rest = torch.tensor([0.5, -0.5, 0.25, 0.1])
+    t = 2.0
+    q = torch.softmax(z.double() / t, 1)
+    tau = torch.where(i < 0, -inf, v.double() / t)
+    p = torch.softmax(torch.cat([tau, rest.double()[:, None]], 1), 1)
+    grad = torch.where(i < 0, 0.0, t * (q - p[:, :4]))   # entry k is class k in every row
+    grad[3, 3] = t * (q[3, 3] - p[3, 4])                 # the last row is an open one
+    return z, v, i, rest, t, grad
+
+
+def test_distill_loss_nothing_left_outside_the_entries():
+    z, v, i, rest, t, grad = closed_rows()
+    z.requires_grad_(True)
+    loss = ops.distill_loss(z, v, i, rest, t, "none")
+    assert bool((loss[:3] == math.inf).all()) and bool(torch.isfinite(loss[3]))
+    got, = torch.autograd.grad(loss, z, torch.ones(4))
+    assert float((got.double() - grad).abs().max()) <= 2.0 ** -22
+
+
 def test_distill_loss_refusals():
     z, v, i, r = torch.randn(4, 7), torch.randn(4, 2), torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4)
     ops.distill_loss(z, v, i, r)

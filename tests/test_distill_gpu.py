@@ -446,3 +446,16 @@ def test_top_logits_and_distill_loss_captured(dtype, V):
         torch.cuda.synchronize()
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_loss_nothing_left_outside_the_entries(dtype):
+    """Loss inf, gradients by the formula: values below 4 as the type rounds the logits (half a step of 4 eps each, T = 2, slopes
+    of q below 1/4), and once more what it rounds of the result."""
+    from test_distill_cpu import closed_rows
+    z, v, i, rest, t, grad = closed_rows()
+    zl = z.to(DEV, dtype).requires_grad_(True)
+    loss = ops.distill_loss(zl, v.to(DEV), i.to(DEV), rest.to(DEV), t, "none")
+    assert bool((loss[:3] == INF).all()) and bool(torch.isfinite(loss[3]))
+    got, = torch.autograd.grad(loss, zl, torch.ones(4, device=DEV))
+    assert float((got.double().cpu() - grad).abs().max()) <= 4 * torch.finfo(dtype).eps + 2.0 ** -20
