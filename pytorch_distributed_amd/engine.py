@@ -128,7 +128,7 @@ def make_teacher(args, device) -> Optional[Teacher]:
         return None
     model = models.get_model(args.teacher, num_classes=args.num_classes) if args.teacher != "mnist_net" else models.Net()
     if args.teacher_checkpoint:
-        utils.load_checkpoint(args.teacher_checkpoint, model)
+        utils.load_checkpoint(args.teacher_checkpoint, model, restore_amp=False)
     dtype = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}[args.precision]
     if hasattr(model, "set_compute_dtype") and torch.device(device).type == "cuda":
         model.set_compute_dtype(dtype)

@@ -58,9 +58,10 @@ def build_state(model, epoch: int, arch: str, best_acc1: float, optimizer=None, 
 
 
 def load_checkpoint(path: str, model=None, optimizer=None, map_location="cpu", strict: bool = True,
-                    trusted: bool = False) -> dict:
+                    trusted: bool = False, restore_amp: bool = True) -> dict:
     """Load a checkpoint written by ``save_checkpoint`` (or by the reference scripts) and
-    restore model / optimizer / amp state.  Returns the payload (``epoch`` = next epoch).
+    restore model / optimizer / amp state (``restore_amp=False``: not the loss scalers', which belong to the process and not
+    to ``model``).  Returns the payload (``epoch`` = next epoch).
 
     The file is read with the tensors-and-plain-containers loader (``weights_only=True``): the payload
     is tensors, numbers, strings, dicts and lists, so nothing in a checkpoint needs code execution and a
@@ -78,7 +79,7 @@ def load_checkpoint(path: str, model=None, optimizer=None, map_location="cpu", s
         model.load_state_dict(sd, strict=strict)
     if optimizer is not None and "optimizer" in ckpt:
         optimizer.load_state_dict(ckpt["optimizer"])
-    if "amp" in ckpt:
+    if restore_amp and "amp" in ckpt:
         from .. import amp
         amp.load_state_dict(ckpt["amp"])
     return ckpt

@@ -1,0 +1,41 @@
+"""What a teacher must leave alone in the training of its student."""
+import pytest
+import torch
+
+from pytorch_distributed_amd import amp, engine, models, utils
+
+
+def _args(*flags):
+    return engine.build_parser().parse_args(["--num-classes", "10", "--teacher", "resnet18", *flags])
+
+
+@pytest.fixture
+def checkpoint(tmp_path):
+    """A checkpoint as a run without dynamic loss scaling writes it."""
+    torch.manual_seed(5)
+    model = models.get_model("resnet18", num_classes=10)
+    opt = torch.optim.SGD(model.parameters(), 0.1)
+    state = utils.build_state(model, 0, "resnet18", 0.0, opt,
+                              {"loss_scaler0": {"loss_scale": 1.0, "unskipped": 7, "skipped_steps": 3, "dynamic": False}})
+    path = str(tmp_path / "teacher.pth.tar")
+    torch.save(state, path)
+    return path, model
+
+
+def test_loading_a_teacher_leaves_the_loss_scaler(checkpoint):
+    path, saved = checkpoint
+    student = models.Net()
+    opt = torch.optim.SGD(student.parameters(), 0.1)
+    try:
+        amp.initialize(student, opt, opt_level="O1", dtype=torch.float16, verbosity=0)
+        before = amp.state_dict()
+        assert before["loss_scaler0"]["dynamic"] and before["loss_scaler0"]["loss_scale"] > 1.0
+        teacher = engine.make_teacher(_args("--teacher-checkpoint", path), "cpu")
+        assert amp.state_dict() == before
+        for a, b in zip(teacher.model.state_dict().values(), saved.state_dict().values()):
+            assert torch.equal(a, b)
+        # --resume still restores it
+        utils.load_checkpoint(path, models.get_model("resnet18", num_classes=10))
+        assert not amp.state_dict()["loss_scaler0"]["dynamic"]
+    finally:
+        amp.initialize(models.Net(), opt_level="O0", verbosity=0)
