@@ -178,7 +178,7 @@ def train(loader, model, criterion, optimizer, epoch: int, device, args, zero_gr
     graph_ddp = _graphable_ddp(model) if _world() > 1 else None
     use_graph = (getattr(args, "graph", False) and torch.device(device).type == "cuda"
                  and (_world() == 1 or graph_ddp is not None) and _takes_metrics(criterion))
-    gstate = getattr(optimizer, "_pda_graph_state", None) if use_graph else None
+    gstate = _graph_state(optimizer, teacher, device) if use_graph else None
     metrics = gstate["metrics"] if gstate is not None else utils.DeviceMetrics(device)
     metrics.reset()
     if use_graph and hasattr(optimizer, "sync_hyperparameters"):
@@ -212,7 +212,8 @@ def train(loader, model, criterion, optimizer, epoch: int, device, args, zero_gr
         images = images.to(device, non_blocking=True)
         target = target.to(device, non_blocking=True)
         if use_graph and gstate is None:
-            gstate = {"metrics": metrics, "x": images.clone(), "t": target.clone(), "eager": 0, "graph": None}
+            gstate = {"metrics": metrics, "x": images.clone(), "t": target.clone(), "eager": 0, "graph": None,
+                      "loss": _loss_constants(teacher)}
             optimizer._pda_graph_state = gstate
         if gstate is not None and images.shape == gstate["x"].shape and target.shape == gstate["t"].shape:
             gstate["x"].copy_(images, non_blocking=True)
@@ -245,6 +246,22 @@ def train(loader, model, criterion, optimizer, epoch: int, device, args, zero_gr
             if jsonl is not None and _rank() == 0:
                 jsonl.log(epoch=epoch, step=i, loss=l, acc1=a1, acc5=a5, images_per_sec=thr.val)
     return losses.avg, top1.avg
+
+
+def _loss_constants(teacher: Optional[Teacher]):
+    """What a recorded step holds of its teacher (the objects themselves, so that none of them can be mistaken for a later one)."""
+    return None if teacher is None else (teacher, teacher.model, teacher.k, teacher.temperature, teacher.weight)
+
+
+def _graph_state(optimizer, teacher: Optional[Teacher], device):
+    """The optimizer's recorded step, or None where nothing has been recorded.  A step of another loss is dropped: eager steps
+    follow, and the new step is recorded after them."""
+    gstate = getattr(optimizer, "_pda_graph_state", None)
+    if gstate is not None and gstate["loss"] != _loss_constants(teacher):
+        if torch.device(device).type == "cuda":
+            torch.cuda.synchronize(device)   # no replay is under way
+        gstate.update(graph=None, eager=0, loss=_loss_constants(teacher))
+    return gstate
 
 
 def _graphable_ddp(model):

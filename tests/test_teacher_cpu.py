@@ -39,3 +39,38 @@ def test_loading_a_teacher_leaves_the_loss_scaler(checkpoint):
         assert not amp.state_dict()["loss_scaler0"]["dynamic"]
     finally:
         amp.initialize(models.Net(), opt_level="O0", verbosity=0)
+
+
+def test_recorded_steps_of_another_teacher_are_dropped():
+    """What a recorded step holds of a teacher as constants is compared with the call's, by value where it may be changed in place."""
+    class Opt:
+        pass
+
+    def recorded(teacher):
+        opt._pda_graph_state = {"graph": Graph(), "eager": 3, "loss": engine._loss_constants(teacher), "metrics": None}
+        opt.gone = False
+
+    class Graph:
+        def __del__(self):
+            opt.gone = True
+
+    def dropped(teacher):
+        g = engine._graph_state(opt, teacher, "cpu")
+        assert g is opt._pda_graph_state
+        assert (g["graph"] is None) == opt.gone == (g["eager"] == 0)
+        assert g["loss"] == engine._loss_constants(teacher)
+        return opt.gone
+
+    opt = Opt()
+    assert engine._graph_state(opt, None, "cpu") is None
+    a, b = engine.Teacher(models.Net()), engine.Teacher(models.Net())
+    for was, now, drop in [(None, None, False), (a, a, False), (None, a, True), (a, None, True), (a, b, True)]:
+        recorded(was)
+        assert dropped(now) == drop
+        assert not drop or engine._graph_state(opt, now, "cpu")["graph"] is None
+    for name, value in [("weight", 0.25), ("k", 8), ("temperature", 1.0), ("model", models.Net())]:
+        recorded(a)
+        setattr(a, name, value)
+        assert dropped(a)
+        recorded(a)
+        assert not dropped(a)
