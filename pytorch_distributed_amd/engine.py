@@ -126,7 +126,10 @@ def make_teacher(args, device) -> Optional[Teacher]:
     """The teacher that ``--teacher`` asks for, or None.  It reads the same batches as the student, with the same head."""
     if not getattr(args, "teacher", ""):
         return None
-    model = models.get_model(args.teacher, num_classes=args.num_classes) if args.teacher != "mnist_net" else models.Net()
+    # its weights come from --seed alone: every rank has the same teacher, and the random state stays the student's
+    with torch.random.fork_rng(devices=[]):
+        torch.default_generator.manual_seed(args.seed or 0)
+        model = models.get_model(args.teacher, num_classes=args.num_classes) if args.teacher != "mnist_net" else models.Net()
     if args.teacher_checkpoint:
         utils.load_checkpoint(args.teacher_checkpoint, model, restore_amp=False)
     dtype = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}[args.precision]

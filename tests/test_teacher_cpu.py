@@ -74,3 +74,15 @@ def test_recorded_steps_of_another_teacher_are_dropped():
         assert dropped(a)
         recorded(a)
         assert not dropped(a)
+
+
+def test_a_teacher_without_a_checkpoint_is_the_same_everywhere():
+    """Every rank builds its own: the weights must not hang on a rank's random state, and that state is left to the student."""
+    made = []
+    for seed, flags in [(1, ()), (2, ()), (3, ("--seed", "9"))]:
+        torch.manual_seed(seed)
+        state = torch.get_rng_state()
+        made.append(engine.make_teacher(_args(*flags), "cpu").model.state_dict())
+        assert torch.equal(torch.get_rng_state(), state)
+    same = [all(torch.equal(made[0][k], m[k]) for k in made[0]) for m in made]
+    assert same == [True, True, False]
