@@ -139,16 +139,20 @@ class GroupNorm(tnn.Module):
         if num_groups <= 0:
             raise ValueError("num_groups must be positive")
 
+        done = {}   # a module of several names stays one
+
         def converted(m: BatchNorm2d) -> "GroupNorm":
-            g = cls(math.gcd(num_groups, m.num_features), m.num_features, m.eps, m.affine)
-            if m.affine:
-                g.weight, g.bias = m.weight, m.bias
-            return g.train(m.training)
+            if m not in done:
+                g = cls(math.gcd(num_groups, m.num_features), m.num_features, m.eps, m.affine)
+                if m.affine:
+                    g.weight, g.bias = m.weight, m.bias
+                done[m] = g.train(m.training)
+            return done[m]
 
         if isinstance(module, BatchNorm2d):
             return converted(module)
         for parent in list(module.modules()):
-            for name, m in list(parent.named_children()):
+            for name, m in list(parent._modules.items()):
                 if isinstance(m, BatchNorm2d):
                     setattr(parent, name, converted(m))
             if hasattr(parent, "fuse_relu_backward"):

@@ -145,3 +145,15 @@ def test_group_norm_act_no_gradient_on_a_border(act, border):
         out = ops.group_norm_act(leaves[0], 2, leaves[1], leaves[2], leaves[3], act)
         assert torch.equal(out, torch.full_like(out, border))
         assert not any(bool(t.any()) for t in torch.autograd.grad(out, leaves, dy))
+
+
+def test_convert_group_norm_of_a_module_with_two_names():
+    """A BatchNorm that two parents (or one parent twice) hold becomes one GroupNorm everywhere."""
+    from pytorch_distributed_amd import nn as pnn
+    bn = pnn.BatchNorm2d(8)
+    m = torch.nn.Module()
+    m.first, m.again, m.inner = bn, bn, torch.nn.Sequential(bn, pnn.BatchNorm2d(8))
+    pnn.GroupNorm.convert_group_norm(m, 4)
+    assert not any(isinstance(k, pnn.BatchNorm2d) for k in (m.first, m.again, *m.inner))
+    assert m.first is m.again is m.inner[0] and m.inner[1] is not m.first
+    assert m.first.weight is bn.weight and m.first.num_groups == 4
