@@ -252,11 +252,15 @@ class ResNet(tnn.Module):
     def _stem(self, images: torch.Tensor) -> torch.Tensor:
         if not isinstance(self.bn1, pnn.BatchNorm2d):   # group norm: the layers one by one
             x = images
-            if self._in_mean is not None or self.input_scale != 1.0:
-                x = x.float() * self.input_scale
-            if self._in_mean is not None:
-                x = (x - self._in_mean.view(1, -1, 1, 1)) * self._in_inv_std.view(1, -1, 1, 1)
-            x = pnn.to_nhwc(x.to(self.compute_dtype))
+            if x.is_cuda and x.dtype in (torch.uint8, torch.float16, torch.float32) and not x.requires_grad:
+                x = ops.input_to_nhwc(x, self.compute_dtype, x.shape[1], mean=self._in_mean, inv_std=self._in_inv_std,
+                                      pre_scale=self.input_scale)
+            else:
+                if self._in_mean is not None or self.input_scale != 1.0:
+                    x = x.float() * self.input_scale
+                if self._in_mean is not None:
+                    x = (x - self._in_mean.view(1, -1, 1, 1)) * self._in_inv_std.view(1, -1, 1, 1)
+                x = pnn.to_nhwc(x.to(self.compute_dtype))
             return self.maxpool(self.bn1(self.conv1(x), None, True))
         return ops.stem_conv_bn_relu_pool(images, self.conv1.weight, self.bn1.weight, self.bn1.bias, self.conv1.stride,
                                           self.conv1.padding, self.bn1.state(), self.compute_dtype,

@@ -57,3 +57,26 @@ def test_student_and_teacher_step_recorded(dtype):
         for p, a, b in zip(params, got[1:], want[1:]):
             # weight gradients of the convolutions are summed in an order that varies
             assert float((a - b).norm()) <= 2e-2 * float(b.norm()) + 1e-5, p.shape
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("given", [torch.uint8, torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("norm", [False, True])
+def test_group_norm_stem_input(dtype, given, norm, monkeypatch):
+    """The stem's input in one pass, and with a gradient to the images by single steps (bf16 images likewise).  An element may differ by
+    two roundings to fp32 and then by one step of the type, d; a sum of 147 of them is some 12 times its own spread, so the
+    normalised output by 12 d and the sums' own 147 roundings."""
+    torch.manual_seed(3)
+    m = pnn.GroupNorm.convert_group_norm(models.resnet18(), 32).to(DEV).set_compute_dtype(dtype)
+    if norm:
+        m.set_input_normalization([0.4, 0.5, 0.6], [0.2, 0.3, 0.25], 1 / 255.0)
+    x = torch.randint(0, 256, (3, 3, 40, 38), device=DEV).to(given)
+    single = []
+    monkeypatch.setattr(pnn, "to_nhwc", lambda t, f=pnn.to_nhwc: (single.append(t), f(t))[1])
+    got = m._stem(x)
+    assert bool(single) == (given is torch.bfloat16)
+    xl = x.float().requires_grad_(True)
+    want = m._stem(xl)
+    assert torch.autograd.grad(want.float().square().sum(), xl)[0].abs().sum() > 0
+    d = max(torch.finfo(dtype).eps, 2.0 ** -22)
+    assert float((got - want).float().norm()) <= (12 * d + 147 * 2.0 ** -24) * float(want.float().norm())
