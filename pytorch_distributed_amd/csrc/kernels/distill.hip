@@ -3,9 +3,13 @@
 //
 // Rows have one stride, their elements are adjacent; a row starts anywhere (odd class counts).  The 16-byte accesses are
 // typed as element-aligned; where a row is written, its first elements are taken alone up to the next 16 bytes.  (Where one is
-// summed up they are not: that costs 5 % on rows of 50001 16-bit classes, but sums do not depend on where a tensor lies.)  One block takes one row; sums of a row's terms are fp32 over a few hundred elements a
-// thread, what the loss is made of (k entries and three log-sum-exps a row) is fp64: student and teacher are nearly equal
-// late in training and their logarithms cancel.
+// summed up they are not: that costs 5 % on rows of 50001 16-bit classes, but sums do not depend on where a tensor lies.)
+//
+// One block takes one row.  Sums S of a row's exponentials are fp32: a thread adds V/256 terms (512 at 131072 classes, 4096 at
+// 2^20), N = 4 or 8 of a vector first, so S is off by at most (V/(256 N) + N + 16) 2^-24 of itself - 5e-6 at 131072 16-bit
+// classes - and as a rule by the root of so many roundings; each term is good to some 2^-22, and c = log2(e)/T, rounded once, acts as
+// a T off by 2^-24 of itself.  That is what bounds the loss (T^2 times it) of a student that has nearly become its teacher.  What
+// is formed from S, the k entries and their log-sum-exps is fp64: logarithms that cancel add nothing to it.
 #include "common.h"
 
 #include <float.h>
@@ -61,6 +65,8 @@ template <typename T> __device__ __forceinline__ float fast_exp2(float x) {
 // multiply-add an element.  mc is the rounded product of the maximum and c; flush() takes its rounding out of the sum.  Where
 // the product is so large that its rounding matters by itself (masks of the type's lowest value, tiny temperatures), and
 // where a NaN or +inf came by, the sum is given as NaN: the caller then looks again with ms_add, which takes differences first.
+// So does a thread that meets nothing but large finite masks (below about -1e9) in its first vectors, at most temperatures: the
+// exponent of such a term is the rounding of mc, and where that overflows the sum stays no number.
 struct FastSum {
   float m = -INFINITY, mc = 0.f, s = 0.f;
   template <int N> __device__ __forceinline__ void add(const float (&z)[N], float c) {
@@ -243,7 +249,8 @@ __device__ MaxSum top_by_digits(const T* row, int V, int K, float c, TopShared& 
 // 4096 rows of 131072 bf16, K = 64: 211 us = 5.1 TB/s, bound by memory; one row 16 us, bound by one CU's bandwidth and the
 // latency of the steps after the read: some 11 000 cycles a block, of which counting ranks takes 2700, the bound 2700 and the
 // second reading 2000 to 4000 (400 x 1000 fp32 7 us, 16384 x 8000 fp16 107 us = 2.5 TB/s).  8 loads are in flight.
-// Rows that do not fit this (more candidates than MAX_CAND: many equal values, K near the number of threads) go digit by digit.
+// Rows that do not fit this (more candidates than MAX_CAND: many equal values, K near the number of threads or above it) go
+// digit by digit: K = 600 takes 4096 x 131072 bf16 4.8 ms.
 template <typename T, int NT, int CELLS>
 __global__ void __launch_bounds__(NT)
 top_logits_kernel(const T* __restrict__ z, long long ld, int V, int K, float c, double temperature, T* __restrict__ values,
@@ -510,7 +517,7 @@ struct RowEntries {
 };
 inline size_t row_entries_bytes(int K, int V) { return 20ull * K + 4ull * ((V + 31) / 32) + 16; }
 
-// One block a row, one read of it: 8192 x 131072 bf16 383 us = 5.6 TB/s, bound by memory; 400 x 1000 by the latency of the row's
+// One block a row, one read of it: 8192 x 131072 bf16 375 us = 5.7 TB/s, bound by memory; 400 x 1000 by the latency of the row's
 // few fp64 steps, which one wave takes.  With rest, classes that are entries stay out of (m, s): the student's remainder is summed by itself, since one minus
 // the entries' sum would keep no digits where the entries hold nearly everything.
 template <typename T, int NT>
@@ -663,7 +670,7 @@ distill_fwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
 }
 
 // dz of a row: one value for every class, then the entries' own over it (the barrier orders the two writes).  Bound by memory:
-// 8192 x 131072 bf16 785 us = 5.5 TB/s.
+// 8192 x 131072 bf16 778 us = 5.5 TB/s.
 // Rows go from the last to the first: what the forward pass read last is still in the memory-side cache, and a gradient too
 // large to stay there itself passes it by (stream: non-temporal stores; 2047 x 50001 bf16 160 -> 144 us with the forward pass,
 // 8192 x 131072 1250 -> 1212 us).
@@ -718,7 +725,7 @@ distill_bwd_kernel(const T* __restrict__ z, long long ld, int V, const void* __r
   }
 }
 
-// out = scale * sum of x: one block, fp64.
+// out = scale * sum of x: one block, fp64 (8192 rows 5.6 us, 2^20 rows 288 us).
 __global__ void __launch_bounds__(1024)
 row_total_kernel(const float* __restrict__ x, long long n, double scale, float* __restrict__ out) {
   __shared__ double red[16];

@@ -140,6 +140,7 @@ __device__ __forceinline__ void gn_dx_coefs(float A, float B, const GnStat& s, f
   pa = -A * r - (float)(s.mean - (double)(float)s.mean) * pb;
 }
 
+// With the hardware's 2^x and 1/x: some 2^-22 in all, nothing to a 16-bit result and four steps of an fp32 one.
 __device__ __forceinline__ float gn_sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
 }

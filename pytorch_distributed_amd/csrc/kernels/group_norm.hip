@@ -87,7 +87,8 @@ gn_partial_kernel(const T* __restrict__ x, long long S, int C, int G, int chunks
   }
 }
 
-// One wave per (sample, group): chunks x D sums -> {mu, r} in fp64.
+// One wave per (sample, group): chunks x D sums -> {mu, r} in fp64.  5 us for 32 groups a sample; one wide group is a long walk (one
+// group of 128x14x14x1024 fp16 68 us, of 1x56x56x256 64, and as much again backward), more than the passes beside it.
 template <typename T>
 __global__ void __launch_bounds__(64)
 gn_finalize_kernel(const T* __restrict__ x, const GnPair* __restrict__ part, long long S, int C, int G, int chunks, double eps,
@@ -152,7 +153,8 @@ gn_apply_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restric
   }
 }
 
-// Per-channel {sum g, sum g xh} of one row chunk of one sample -> part[n][chunk][c].
+// Per-channel {sum g, sum g xh} of one row chunk of one sample -> part[n][chunk][c].  fp32 over a thread's rows and the block's
+// tree; what joins chunks, channels and samples is fp64.
 template <typename T, int VEC, bool UG, int ACT>
 __global__ void __launch_bounds__(256)
 gn_bwd_partial_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ dout,
@@ -259,8 +261,8 @@ gn_bwd_finalize_kernel(const float2* __restrict__ part, const float* __restrict_
 
 // dgamma_c, dbeta_c: the column sums of part [rows][C].  A block takes 4 channels with 256 lanes of rows each: with one
 // block a channel group the walk over the rows (thousands at large batch) has to be short.  Many rows are summed in two
-// steps: blockIdx.y takes `span` rows and leaves their sums in the first of them, which no other block reads; the second
-// step (dbeta given) takes those, `step` rows apart.
+// steps: blockIdx.y takes `span` rows and leaves their sums in the first of them (rounded to fp32 there, 2^-24 of each), which no
+// other block reads; the second step (dbeta given) takes those, `step` rows apart.
 __global__ void __launch_bounds__(1024)
 gn_params_kernel(float2* part, long long rows, long long span, long long step, int C, float* __restrict__ dgamma,
                  float* __restrict__ dbeta) {

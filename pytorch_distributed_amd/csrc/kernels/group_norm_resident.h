@@ -32,7 +32,7 @@ inline size_t gn_bwd_lds(int W, int threads, int vec, int D) {
 }
 
 // Measured on 400 samples, fp16, forward / backward: the width of a slab's rows counts most (56x56x256 with residual:
-// 16 bytes 701 / 1381 us, 32 bytes 530 / 941, 64 bytes 441 / 736: 4.4 TB/s), up to 128 bytes (14x14x1024: 32 bytes 114 / 202, 64 bytes
+// 16 bytes 701 / 1381 us, 32 bytes 530 / 941, 64 bytes 441 / 736 next to each other; on its own 472 / 781 = 4.1 TB/s), up to 128 bytes (14x14x1024: 32 bytes 114 / 202, 64 bytes
 // 101 / 183, 128 bytes 108 / 194), then few threads with many vectors (28x28x512: 512 threads 197, 1024 230 us).
 inline GnPlan gn_resident_plan(int esize, long long N, long long S, int C, int G, bool bwd) {
   GnPlan best{0, 0, 0};
