@@ -179,7 +179,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, gamma: Optional[torch.Tenso
     The mean and the variance are those of one sample's ``C / num_groups`` adjacent channels at all its positions.
     ``act``: ``False`` (none), ``True`` (ReLU), a positive number (ReLU clipped there, 6 for ReLU6) or ``"silu"``.
     ``gamma`` and ``beta`` (``[C]``, both or neither) keep their own dtype.  Differentiable once, in ``x``, ``gamma``,
-    ``beta`` and ``residual``; a sample whose values hold a NaN or an infinity gives NaN in that group."""
+    ``beta`` and ``residual``; a sample whose values hold a NaN or an infinity gives NaN in that group.  Gradients are those of
+    deviations (``sqrt(var + eps)``) between 1e-18 and 1e18, whose squares fp32 holds."""
     eps = float(eps)
     groups = _check(x, num_groups, gamma, beta, residual, eps)
     code, cap = _act_code(act)

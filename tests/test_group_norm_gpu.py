@@ -12,6 +12,7 @@ from pytorch_distributed_amd import ops
 
 DEV = "cuda"
 U = 2.0 ** -24
+INF = float("inf")
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 # least difference that the type can show
 TINY = {torch.float32: 1e-40, torch.float16: 2.0 ** -25, torch.bfloat16: 1e-38}
@@ -270,6 +271,29 @@ def test_group_norm_act_constant_groups_and_nan():
     assert bool(bad[1, :, :, 4:8].all()) and int(bad.sum()) == 6 * 6 * 4
     x[1, 2, 3, 5] = float("inf")
     assert int(torch.isnan(ops.group_norm_act(x, 4, w, b, None, "silu")).sum()) == 6 * 6 * 4
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,groups", [((2, 6, 6, 32), 4), ((2, 14, 14, 48), 8), ((3, 6, 6, 58), 2), ((2, 120, 120, 24), 3)])
+def test_group_norm_act_no_number_in_first_place(shape, groups, dtype):
+    """The first value of a group, from which its sums are taken, and the last one: NaN in that group alone, the others as before."""
+    x, w, b, _, dy = make(shape, dtype, 53)
+    D = shape[-1] // groups
+    leaf = x.clone().requires_grad_(True)
+    ref = ops.group_norm_act(leaf, groups, w, b, None, "silu")
+    dref, = torch.autograd.grad(ref, leaf, dy)
+    for bad in (float("nan"), INF, -INF):
+        for at in ((1, 0, 0, D), (1, shape[1] - 1, shape[2] - 1, 2 * D - 1)):
+            y = x.clone()
+            y[at] = bad
+            y.requires_grad_(True)
+            out = ops.group_norm_act(y, groups, w, b, None, "silu")
+            dx, = torch.autograd.grad(out, y, dy)
+            for got, was in ((out, ref), (dx, dref)):
+                assert bool(got[1, ..., D:2 * D].isnan().all())
+                keep = torch.ones_like(got, dtype=torch.bool)
+                keep[1, ..., D:2 * D] = False
+                assert torch.equal(got[keep], was[keep])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
